@@ -252,6 +252,45 @@ int nk_fused(nk_dev dev, const int32_t* program, int n_ops, const double* consts
              int dtype, int rank, nk_buf drn, const int32_t* drn_cfg,
              int n_src, const nk_buf* srcs, const int32_t* const* src_cfgs, int64_t n);
 
+/* ---- the operators of a feed-forward sublayer, forward and backward.  No counterpart in the reference, which composes them of
+ *      matMul, broadcasts and activations.  All buffers are dense unless a pitch says otherwise; no output may overlap an input
+ *      except where that is said. */
+
+/* Layer normalisation of `rows` rows of `cols` elements; row i of `src` starts at element i * src_pitch (src_pitch >= cols).
+ *     drn = (src - mean) * rstd * gain + bias,  rstd = 1 / sqrt(variance + epsilon)  (gain and bias: `cols` elements each)
+ * mean and rstd (`rows` elements each, both or neither 0) are written for the backward pass.  drn may be src where
+ * src_pitch == cols. */
+int nk_layer_norm(nk_dev dev, int dtype, int64_t rows, int64_t cols, nk_buf src, int64_t src_pitch, nk_buf gain, nk_buf bias,
+                  double epsilon, nk_buf drn, nk_buf mean, nk_buf rstd);
+/* Its gradients for the error of drn: d_src (dense, rows x cols), d_gain and d_bias (`cols` elements); any of them may be 0
+ * (not wanted).  src, gain, mean and rstd are those of the forward call.  The sums over the rows are added in an order that depends
+ * on the shape alone. */
+int nk_layer_norm_backward(nk_dev dev, int dtype, int64_t rows, int64_t cols, nk_buf src, int64_t src_pitch, nk_buf gain, nk_buf mean,
+                           nk_buf rstd, nk_buf error, nk_buf d_src, nk_buf d_gain, nk_buf d_bias);
+
+/* Dropout: drn[i] = keep(i) ? src[i] / (1 - probability) : 0 for every i of a view, n elements (drn may be src).
+ * keep(i): word i % 4 of Philox4x32-10 with key = seed and counter = (i / 4, offset) is at least floor(probability * 2^32), i the
+ * row-major index.  No mask is stored: the backward pass is the same call on the error.  Calls that shall draw
+ * independently differ in seed or offset. */
+int nk_dropout(nk_dev dev, int dtype, int rank, nk_buf drn, const int32_t* drn_cfg, nk_buf src, const int32_t* src_cfg,
+               double probability, uint64_t seed, uint64_t offset, int64_t n);
+
+/* The gated half of a feed-forward block in one pass over its input:
+ *     gate = X @ Wg,  up = X @ Wu,  drn = f(gate) * up      X[M,K], Wg and Wu [K,N], drn[M,N]
+ * f is one of NK_FUN_IDY, RELU, SIG, SILU, GELU, TANH.  weight_layout: NK_LAYOUT_ROW_MAJOR, or NK_LAYOUT_COLUMN_MAJOR for weights
+ * stored as [N,K]; everything else is row-major.  gate and up ([M,N], both or neither 0) are written for the backward pass.
+ * Element types: f64 products run on the f64 matrix cores.  f32 operands enter the matrix cores as sums of three bfloat16 numbers
+ * (24 bits, exactly the operand's where its magnitude is 2^-110 or more), every product as the six partial products above
+ * 2^-24 of it, added in f32: the error stays within 1e-5 of sum_k |x_ik| |w_kj| like that of nk_matmul, and infinities and NaN
+ * give what f32 arithmetic gives.  Every sum is added in an order that depends on shape and layout alone. */
+int nk_gated_matmul(nk_dev dev, int fun_id, int dtype, int weight_layout, int64_t M, int64_t K, int64_t N, nk_buf X, nk_buf Wg, nk_buf Wu,
+                    nk_buf drn, nk_buf gate, nk_buf up);
+/* Its gradients for the error of drn ([M,N]), with gate and up of the forward call:
+ *     dg = error * up * f'(gate),  du = error * f(gate),  d_X = dg @ Wg^T + du @ Wu^T,  d_Wg = X^T @ dg,  d_Wu = X^T @ du
+ * d_X [M,K], d_Wg and d_Wu [K,N] (row-major whatever weight_layout is); d_X may be 0, d_Wg and d_Wu both or neither. */
+int nk_gated_matmul_backward(nk_dev dev, int fun_id, int dtype, int weight_layout, int64_t M, int64_t K, int64_t N, nk_buf X, nk_buf Wg,
+                             nk_buf Wu, nk_buf gate, nk_buf up, nk_buf error, nk_buf d_X, nk_buf d_Wg, nk_buf d_Wu);
+
 #ifdef __cplusplus
 }
 #endif

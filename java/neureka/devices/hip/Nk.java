@@ -58,6 +58,13 @@ public final class Nk {
     public static final MethodHandle nk_dot               = h("nk_dot", I, J, I, J, J, J, J);
     public static final MethodHandle nk_fused             = h("nk_fused", I, J, P, I, P, I, I, I, J, P, I, P, P, J);
 
+    // the operators of a feed-forward sublayer
+    public static final MethodHandle nk_layer_norm        = h("nk_layer_norm", I, J, I, J, J, J, J, J, J, D, J, J, J);
+    public static final MethodHandle nk_layer_norm_backward = h("nk_layer_norm_backward", I, J, I, J, J, J, J, J, J, J, J, J, J, J);
+    public static final MethodHandle nk_dropout           = h("nk_dropout", I, J, I, I, J, P, J, P, D, J, J, J);
+    public static final MethodHandle nk_gated_matmul      = h("nk_gated_matmul", I, J, I, I, I, J, J, J, J, J, J, J, J, J);
+    public static final MethodHandle nk_gated_matmul_backward = h("nk_gated_matmul_backward", I, J, I, I, I, J, J, J, J, J, J, J, J, J, J, J, J);
+
     /** Runs a downcall that returns a status; a non-zero status becomes the exception the caller expects. */
     public interface Call { int run() throws Throwable; }
     public static void check(Call c) {

@@ -62,6 +62,11 @@ SYMBOLS = {
     "nk_dot": (_i32, [_u64, _i32, _u64, _u64, _i64, _u64]),
     "nk_fused": (_i32, [_u64, C.POINTER(C.c_int32), _i32, C.POINTER(C.c_double), _i32, _i32, _i32, _u64, _cfg, _i32,
                         C.POINTER(_u64), C.POINTER(_cfg), _i64]),
+    "nk_layer_norm": (_i32, [_u64, _i32, _i64, _i64, _u64, _i64, _u64, _u64, C.c_double, _u64, _u64, _u64]),
+    "nk_layer_norm_backward": (_i32, [_u64, _i32, _i64, _i64, _u64, _i64, _u64, _u64, _u64, _u64, _u64, _u64, _u64]),
+    "nk_dropout": (_i32, [_u64, _i32, _i32, _u64, _cfg, _u64, _cfg, C.c_double, _u64, _u64, _i64]),
+    "nk_gated_matmul": (_i32, [_u64, _i32, _i32, _i32, _i64, _i64, _i64, _u64, _u64, _u64, _u64, _u64, _u64]),
+    "nk_gated_matmul_backward": (_i32, [_u64, _i32, _i32, _i32, _i64, _i64, _i64, _u64, _u64, _u64, _u64, _u64, _u64, _u64, _u64, _u64]),
 }
 
 

@@ -36,6 +36,7 @@ class ExecutionCall:
     inputs: List[Optional[object]]
     derivIdx: int = -1
     algorithm: Optional["Algorithm"] = None
+    args: Dict[str, object] = field(default_factory=dict)     # further arguments by name (math/args/Args.java)
 
     def input(self, i: int):
         return self.inputs[i]
@@ -50,15 +51,15 @@ class ExecutionCall:
     def withInputAt(self, i: int, t) -> "ExecutionCall":
         inputs = list(self.inputs)
         inputs[i] = t
-        return ExecutionCall(self.device, self.operation, inputs, self.derivIdx, self.algorithm)
+        return ExecutionCall(self.device, self.operation, inputs, self.derivIdx, self.algorithm, self.args)
 
     def withAddedInputAt(self, i: int, t) -> "ExecutionCall":
         inputs = list(self.inputs)
         inputs.insert(i, t)
-        return ExecutionCall(self.device, self.operation, inputs, self.derivIdx, self.algorithm)
+        return ExecutionCall(self.device, self.operation, inputs, self.derivIdx, self.algorithm, self.args)
 
     def withInputs(self, inputs: Sequence) -> "ExecutionCall":
-        return ExecutionCall(self.device, self.operation, list(inputs), self.derivIdx, self.algorithm)
+        return ExecutionCall(self.device, self.operation, list(inputs), self.derivIdx, self.algorithm, self.args)
 
 
 class Algorithm:
@@ -372,6 +373,96 @@ class DotProductAlgorithm(Algorithm):
         return call.withInputs(ins)
 
 
+def _one_type(what: str, tensors) -> None:
+    if any(t.dtype != tensors[0].dtype for t in tensors):
+        raise IllegalArgumentException(f"the operands of {what} are of one type, got {', '.join(str(t.dtype) for t in tensors)}")
+
+
+def as_rows(t):
+    """The tensor itself where its last axis is contiguous and its rows lie one pitch apart, else a dense copy."""
+    if t.isVirtual():
+        t.setIsVirtual(False)
+    return t if t.ndc.asRows() is not None else t.deepCopy()
+
+
+def as_dense(t):
+    """The tensor itself where its elements lie next to each other in row-major order, else a dense copy."""
+    if t.isVirtual():
+        t.setIsVirtual(False)
+    return t if t.ndc.asDense() is not None else t.deepCopy()
+
+
+class LayerNormAlgorithm(Algorithm):
+    """Normalisation over the last axis: (drain, source, gain, bias), ``epsilon`` by name.  A call whose graph is recorded
+    (``keep``) also keeps mean and reciprocal deviation of every row."""
+    name = "layer_norm"
+
+    def isSuitableFor(self, call):
+        return GOOD
+
+    def prepare(self, call):
+        src, gain, bias = call.inputs
+        _one_type("layerNorm", call.inputs)
+        cols = src.shape[-1]
+        for what, t in (("gain", gain), ("bias", bias)):
+            if t.shape[-1] != cols or t.size != cols:
+                raise IllegalArgumentException(f"the {what} of layerNorm has shape {list(t.shape)}, the last axis of the source {cols} elements")
+        if not 0 <= call.args["epsilon"] < float("inf"):
+            raise IllegalArgumentException(f"the epsilon of layerNorm is finite and not negative, not {call.args['epsilon']}")
+        src, gain, bias = as_rows(src), as_dense(gain), as_dense(bias)
+        if call.args.get("keep"):
+            rows = src.size // cols
+            call.args["mean"], call.args["rstd"] = (call.device.allocate(src.dtype, rows) for _ in range(2))
+        return call.withInputs([_new_output(call.device, src.dtype, src.shape, overwritten=True), src, gain, bias])
+
+
+class DropoutAlgorithm(Algorithm):
+    """(drain, source); ``probability``, ``seed`` and ``offset`` by name."""
+    name = "dropout"
+
+    def isSuitableFor(self, call):
+        return GOOD
+
+    def prepare(self, call):
+        a = call.args
+        if not 0 <= a["probability"] <= 1:
+            raise IllegalArgumentException(f"the probability of a drop lies in [0, 1], not at {a['probability']}")
+        for what in ("seed", "offset"):
+            if not 0 <= a[what] < 1 << 64:
+                raise IllegalArgumentException(f"the {what} of a dropout is an unsigned 64-bit number, not {a[what]}")
+        src = call.input(0)
+        return call.withInputs([_new_output(call.device, src.dtype, src.shape, overwritten=True), src])
+
+
+class GatedMatMulAlgorithm(Algorithm):
+    """f(x @ gate) * (x @ up): (drain, source [..., K], gate weight [K, N], up weight [K, N]), ``activation`` by name.  A call
+    whose graph is recorded (``keep``) also keeps both products."""
+    name = "gated_matmul"
+
+    def isSuitableFor(self, call):
+        return GOOD
+
+    def prepare(self, call):
+        x, gate, up = call.inputs
+        _one_type("gatedMatMul", call.inputs)
+        if call.args["activation"] not in HipDevice.GATED_ACTIVATIONS:
+            raise IllegalArgumentException(f"gatedMatMul takes one of {', '.join(HipDevice.GATED_ACTIVATIONS)}, not '{call.args['activation']}'")
+        if gate.rank != 2 or gate.shape != up.shape or gate.shape[0] != x.shape[-1]:
+            raise IllegalArgumentException(f"weights {list(gate.shape)} and {list(up.shape)} do not fit rows of {x.shape[-1]}: both are [{x.shape[-1]}, columns]")
+        x = as_dense(x)
+        for w in (gate, up):
+            if w.isVirtual():
+                w.setIsVirtual(False)
+        # both as they lie, by rows or by columns; anything else becomes dense rows
+        if not (all(w.ndc.asDense() is not None for w in (gate, up)) or all(w.ndc.asDenseColumns() is not None for w in (gate, up))):
+            gate, up = as_dense(gate), as_dense(up)
+        shape = x.shape[:-1] + (gate.shape[1],)
+        if call.args.get("keep"):
+            size = x.size // x.shape[-1] * gate.shape[1]
+            call.args["gate"], call.args["up"] = (call.device.allocate(x.dtype, size) for _ in range(2))
+        return call.withInputs([_new_output(call.device, x.dtype, shape, overwritten=True), x, gate, up])
+
+
 class Operation:
     """An operation with its algorithms (backend/api/Operation.java; template/operations/AbstractOperation.java:178-211)."""
 
@@ -444,6 +535,10 @@ class BackendContext:
         for f in ACTIVATIONS:      # functions/AbstractActivationOperation.java:38-50
             self.operations[f] = Operation(f, f, [ElementwiseAlgorithm(), ScalarBroadcast(), ScalarAlgorithm()])
         self.operations["left_inline"] = Operation("left_inline", "<", [AssignScalar(), AssignElementwise()])
+        # the operators of a feed-forward sublayer, which the reference composes of others
+        self.operations["layerNorm"] = Operation("layerNorm", "layerNorm", [LayerNormAlgorithm()])
+        self.operations["dropout"] = Operation("dropout", "dropout", [DropoutAlgorithm()])
+        self.operations["gatedMatMul"] = Operation("gatedMatMul", "gatedMatMul", [GatedMatMulAlgorithm()])
         self.operations["random"] = Operation("random", "rand", [ElementwiseAlgorithm()])
         self.extensions: List[object] = []
 
@@ -636,6 +731,24 @@ def hip_dot(call: ExecutionCall):
     return out
 
 
+def hip_layer_norm(call: ExecutionCall):
+    a = call.args
+    call.device.launch_layer_norm(call.input(0), call.input(1), call.input(2), call.input(3), a["epsilon"], a.get("mean"), a.get("rstd"))
+    return call.input(0)
+
+
+def hip_dropout(call: ExecutionCall):
+    a = call.args
+    call.device.launch_dropout(call.input(0), call.input(1), a["probability"], a["seed"], a["offset"])
+    return call.input(0)
+
+
+def hip_gated_matmul(call: ExecutionCall):
+    a = call.args
+    call.device.launch_gated_matmul(a["activation"], call.input(0), call.input(1), call.input(2), call.input(3), a.get("gate"), a.get("up"))
+    return call.input(0)
+
+
 class HipBackend:
     """``BackendExtension`` for HipDevice (model: backend/ocl/CLBackend.java:56-325)."""
 
@@ -667,6 +780,9 @@ class HipBackend:
         registry.forOperation("min").set(ReduceAlgorithm, hip_reduce("min"))
         registry.forOperation("max").set(ReduceAlgorithm, hip_reduce("max"))
         registry.forOperation("dot").set(DotProductAlgorithm, hip_dot)
+        registry.forOperation("layerNorm").set(LayerNormAlgorithm, hip_layer_norm)
+        registry.forOperation("dropout").set(DropoutAlgorithm, hip_dropout)
+        registry.forOperation("gatedMatMul").set(GatedMatMulAlgorithm, hip_gated_matmul)
         (registry.forOperation("left_inline")                                    # CLBackend.java:232-234
             .set(BiScalarBroadcast, hip_scalar_broadcast_identity)
             .set(ElementwiseAlgorithm, hip_assign_elementwise))

@@ -441,6 +441,119 @@ class HipDevice:
         _lib.check(self._lib.nk_fused(self.handle, prog, len(program) // 2, cs, len(consts), _dtype_code(drn.dtype), drn.ndc.rank,
                                       ops[0][0], ops[0][2], len(srcs), ptrs, cfgs, drn.ndc.size))
 
+    # ---- the operators of a feed-forward sublayer (include/neureka_hip.h) ----------------------------
+    def _dense_at(self, what: str, t, dtype, size: int) -> int:
+        """Address of `size` elements that lie next to each other: a tensor of this device or a bare buffer."""
+        if isinstance(t, HipData):
+            if t.device is not self:
+                raise IllegalStateException(f"{what} is not stored on the executing HipDevice")
+            held, base = t.size, 0
+        else:
+            if t._device is not self:
+                raise IllegalStateException(f"{what} is not stored on the executing HipDevice")
+            held, base = t.ndc.size, None if t._virtual else t.ndc.asDense()
+        if t.dtype != dtype:
+            raise IllegalArgumentException(f"{what} holds {t.dtype}, {np.dtype(dtype)} is needed")
+        if held != size:
+            raise IllegalArgumentException(f"{what} has {held} elements, {size} are needed")
+        if base is None:
+            raise IllegalArgumentException(f"{what} has to be dense (row-major)")
+        return (t.ptr if isinstance(t, HipData) else t._data.ptr) + base * t.dtype.itemsize
+
+    def _rows_at(self, what: str, t):
+        """(address, rows, columns, pitch) of a tensor of this device."""
+        if t._device is not self:
+            raise IllegalStateException(f"{what} is not stored on the executing HipDevice")
+        rows = None if t._virtual else t.ndc.asRows()
+        if rows is None:
+            raise IllegalArgumentException(f"the last axis of {what} has to be contiguous and its rows one pitch apart")
+        return (t._data.ptr + rows[0] * t.dtype.itemsize,) + rows[1:]
+
+    def launch_layer_norm(self, drn, src, gain, bias, epsilon: float = 1e-5, mean=None, rstd=None) -> None:
+        """drn = (src - mean) * rstd * gain + bias over the last axis; `mean` and `rstd` (one element per row) are written where
+        given.  `drn` may be `src`."""
+        dt = drn.dtype
+        code = _dtype_code(dt)
+        at, rows, cols, pitch = self._rows_at("the source", src)
+        if src.dtype != dt or src.shape != drn.shape:
+            raise IllegalArgumentException(f"source {src.dtype}{list(src.shape)} and drain {dt}{list(drn.shape)} differ")
+        _lib.check(self._lib.nk_layer_norm(
+            self.handle, code, rows, cols, at, pitch, self._dense_at("the gain", gain, dt, cols), self._dense_at("the bias", bias, dt, cols),
+            epsilon, self._dense_at("the drain", drn, dt, rows * cols), 0 if mean is None else self._dense_at("mean", mean, dt, rows),
+            0 if rstd is None else self._dense_at("rstd", rstd, dt, rows)))
+
+    def launch_layer_norm_backward(self, src, gain, mean, rstd, error, d_src=None, d_gain=None, d_bias=None) -> None:
+        """The gradients of launch_layer_norm that are asked for, given the error of its drain."""
+        dt = src.dtype
+        code = _dtype_code(dt)
+        at, rows, cols, pitch = self._rows_at("the source", src)
+        outs = [0 if t is None else self._dense_at(what, t, dt, size) for what, t, size in
+                (("d_src", d_src, rows * cols), ("d_gain", d_gain, cols), ("d_bias", d_bias, cols))]
+        _lib.check(self._lib.nk_layer_norm_backward(
+            self.handle, code, rows, cols, at, pitch, self._dense_at("the gain", gain, dt, cols), self._dense_at("mean", mean, dt, rows),
+            self._dense_at("rstd", rstd, dt, rows), self._dense_at("the error", error, dt, rows * cols), *outs))
+
+    def launch_dropout(self, drn, src, probability: float, seed: int, offset: int = 0) -> None:
+        """drn = keep ? src / (1 - probability) : 0, keep from (seed, offset) and the element's row-major index."""
+        for what, v in (("seed", seed), ("offset", offset)):
+            if not 0 <= v < 1 << 64:
+                raise IllegalArgumentException(f"the {what} of a dropout is an unsigned 64-bit number, not {v}")
+        if src.dtype != drn.dtype or src.shape != drn.shape:
+            raise IllegalArgumentException(f"source {src.dtype}{list(src.shape)} and drain {drn.dtype}{list(drn.shape)} differ")
+        if src._device is not self or drn._device is not self:
+            raise IllegalStateException("source or drain is not stored on the executing HipDevice")
+        if drn._virtual:
+            raise IllegalArgumentException("the drain of a dropout has to be an actual tensor")
+        (p0, k0, c0), (p1, k1, c1) = self._ops(drn, src)
+        _lib.check(self._lib.nk_dropout(self.handle, _dtype_code(drn.dtype), drn.ndc.rank, p0, c0, p1, c1, probability, seed, offset, drn.ndc.size))
+
+    GATED_ACTIVATIONS = ("idy", "relu", "sig", "silu", "gelu", "tanh")
+
+    def _gated_operands(self, fun: str, x, gate_weight, up_weight):
+        """Leading arguments of the two gated entry points, and (dtype, M, K, N)."""
+        if fun not in self.GATED_ACTIVATIONS:
+            raise IllegalArgumentException(f"a gated product takes one of {', '.join(self.GATED_ACTIVATIONS)}, not '{fun}'")
+        dt = x.dtype
+        code = _dtype_code(dt)
+        K = x.ndc.shape[-1]
+        M = x.ndc.size // K
+        if gate_weight.rank != 2 or gate_weight.shape != up_weight.shape or gate_weight.shape[0] != K:
+            raise IllegalArgumentException(f"weights {list(gate_weight.shape)} and {list(up_weight.shape)} do not fit rows of {K}: both are [{K}, columns]")
+        N = gate_weight.shape[1]
+        layout, at = _lib.ROW_MAJOR, []
+        both = (("the gate weight", gate_weight), ("the up weight", up_weight))
+        if any(w._virtual or w.ndc.asDense() is None for _, w in both):
+            layout = _lib.COLUMN_MAJOR               # [K, N] as a view of a dense [N, K]
+        for what, w in both:
+            if layout == _lib.ROW_MAJOR:
+                at.append(self._dense_at(what, w, dt, K * N))
+                continue
+            base = None if w._virtual else w.ndc.asDenseColumns()
+            if w._device is not self:
+                raise IllegalStateException(f"{what} is not stored on the executing HipDevice")
+            if w.dtype != dt:
+                raise IllegalArgumentException(f"{what} holds {w.dtype}, {dt} is needed")
+            if base is None:
+                raise IllegalArgumentException("the weights have to be dense, both row-major or both column-major")
+            at.append(w._data.ptr + base * dt.itemsize)
+        return (self.handle, _lib.FUN[fun], code, layout, M, K, N, self._dense_at("the input", x, dt, M * K), at[0], at[1]), dt, M, K, N
+
+    def launch_gated_matmul(self, fun: str, drn, x, gate_weight, up_weight, gate=None, up=None) -> None:
+        """drn = fun(x @ gate_weight) * (x @ up_weight); both products are written to `gate` and `up` where given."""
+        head, dt, M, K, N = self._gated_operands(fun, x, gate_weight, up_weight)
+        _lib.check(self._lib.nk_gated_matmul(
+            *head, self._dense_at("the drain", drn, dt, M * N), 0 if gate is None else self._dense_at("gate", gate, dt, M * N),
+            0 if up is None else self._dense_at("up", up, dt, M * N)))
+
+    def launch_gated_matmul_backward(self, fun: str, x, gate_weight, up_weight, gate, up, error, d_x=None, d_gate_weight=None, d_up_weight=None) -> None:
+        """The gradients of launch_gated_matmul that are asked for (those of the weights both or neither; row-major)."""
+        head, dt, M, K, N = self._gated_operands(fun, x, gate_weight, up_weight)
+        _lib.check(self._lib.nk_gated_matmul_backward(
+            *head, self._dense_at("gate", gate, dt, M * N), self._dense_at("up", up, dt, M * N), self._dense_at("the error", error, dt, M * N),
+            0 if d_x is None else self._dense_at("d_x", d_x, dt, M * K),
+            0 if d_gate_weight is None else self._dense_at("d_gate_weight", d_gate_weight, dt, K * N),
+            0 if d_up_weight is None else self._dense_at("d_up_weight", d_up_weight, dt, K * N)))
+
     def prepared(self, entry: str, *args):
         """Binds one C-ABI call with its arguments converted once; the returned callable repeats exactly
         that launch (used where the per-call cost of building descriptors would distort a measurement).

@@ -19,7 +19,7 @@ from typing import List, Optional, Sequence, Union
 
 from . import _lib
 from .backend import (ACTIVATIONS, BiElementwise, BiScalarBroadcast, Broadcast, ExecutionCall, ScalarAlgorithm,
-                      ScalarBroadcast, backend, execute_device_algorithm, execute_on_common_device)
+                      ScalarBroadcast, as_dense, backend, execute_device_algorithm, execute_on_common_device)
 from .ndim import IllegalArgumentException, IllegalStateException
 from .tensor import GraphNode, Tensor, make_fit
 
@@ -32,7 +32,11 @@ def _device_for(inputs: Sequence[Tensor]):
     raise IllegalStateException("none of the operands is stored on a HipDevice; this package has no host arithmetic path")
 
 
-def execute(op_id: str, inputs: Sequence[Tensor], d: int = -1, record: bool = True) -> Tensor:
+# operations whose operands keep their own ranks and whose gradients come out of one call
+SUBLAYER_OPERATIONS = ("layerNorm", "dropout", "gatedMatMul")
+
+
+def execute(op_id: str, inputs: Sequence[Tensor], d: int = -1, record: bool = True, args: Optional[dict] = None) -> Tensor:
     ctx = backend()
     operation = ctx.getOperation(op_id)
     device = _device_for(inputs)
@@ -41,9 +45,14 @@ def execute(op_id: str, inputs: Sequence[Tensor], d: int = -1, record: bool = Tr
             raise IllegalArgumentException("Assignment does not support autograd!")
         record = False
     parents = list(inputs)                   # the tensors the caller holds: gradients attach to these
-    if len(inputs) > 1 and op_id != "dot" and any(len(t.ndc.shape) != len(inputs[0].ndc.shape) for t in inputs):
+    if op_id in SUBLAYER_OPERATIONS and d >= 0:
+        raise IllegalArgumentException(f"'{op_id}' has no elementwise derivative; its gradients come from backward()")
+    if len(inputs) > 1 and op_id != "dot" and op_id not in SUBLAYER_OPERATIONS and any(len(t.ndc.shape) != len(inputs[0].ndc.shape) for t in inputs):
         inputs = make_fit(list(inputs))      # FunctionNode.execute pads ranks first (FunctionNode.java:92-93)
+    recorded = record and d < 0 and any(t.rqsGradient() or t._node is not None for t in parents)
     call = ExecutionCall(device, operation, list(inputs), d)
+    if args is not None or op_id in SUBLAYER_OPERATIONS:
+        call.args = dict(args or {}, keep=recorded)
     call.algorithm = operation.getAlgorithmFor(call)
 
     def run(c: ExecutionCall):
@@ -54,8 +63,9 @@ def execute(op_id: str, inputs: Sequence[Tensor], d: int = -1, record: bool = Tr
         return execute_device_algorithm(c), c
 
     result, prepared = execute_on_common_device(call, run)
-    if record and d < 0 and any(t.rqsGradient() or t._node is not None for t in parents):
-        result._node = _graph_node(op_id, prepared, parents, result)
+    if recorded:
+        joint = _joint_gradients(op_id, prepared, parents) if op_id in SUBLAYER_OPERATIONS else None
+        result._node = GraphNode(parents, (), joint) if joint else _graph_node(op_id, prepared, parents, result)
     return result
 
 
@@ -69,6 +79,37 @@ def _graph_node(op_id: str, call: ExecutionCall, inputs: List[Tensor], result: T
             continue
         actions.append(_ad_action(op_id, alg, call, inputs, d, result))
     return GraphNode(inputs, actions)
+
+
+def _joint_gradients(op_id: str, call: ExecutionCall, parents: List[Tensor]):
+    """For operations whose gradients share their work: error of the result -> one gradient (or None) per parent."""
+    device, args = call.device, call.args
+    drn, *operands = call.inputs                  # as the kernel saw them
+    shape, dtype = drn.shape, drn.dtype
+    wanted = [t.rqsGradient() or t._node is not None for t in parents]
+
+    def act(error: Tensor) -> List[Optional[Tensor]]:
+        if error.shape != shape or error.dtype != dtype:
+            raise IllegalArgumentException(f"the error of a {dtype}{list(shape)} result cannot be {error.dtype}{list(error.shape)}")
+        # operands that live on the host are stored for the launch and restored afterwards
+        run = ExecutionCall(device, call.operation, operands + [error], args=args)
+        return execute_on_common_device(run, lambda c: gradients(error))
+
+    def gradients(error: Tensor) -> List[Optional[Tensor]]:
+        if op_id == "dropout":
+            return [execute("dropout", [error], record=False, args={k: args[k] for k in ("probability", "seed", "offset")})]
+        error = as_dense(error)
+        out = [Tensor._on_device(device, dtype, p.shape, zeroed=False) if w else None for p, w in zip(parents, wanted)]
+        if op_id == "layerNorm":
+            src, gain, _ = operands
+            device.launch_layer_norm_backward(src, gain, args["mean"], args["rstd"], error, *out)
+            return out
+        d_x, d_gate, d_up = out
+        if (d_gate is None) != (d_up is None):    # the kernel computes both
+            d_gate, d_up = (Tensor._on_device(device, dtype, parents[1].shape, zeroed=False) if t is None else t for t in (d_gate, d_up))
+        device.launch_gated_matmul_backward(args["activation"], *operands, args["gate"], args["up"], error, d_x, d_gate, d_up)
+        return out
+    return act
 
 
 def _ad_action(op_id: str, alg, call: ExecutionCall, inputs: List[Tensor], d: int, result: Optional[Tensor] = None):

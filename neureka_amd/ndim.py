@@ -201,6 +201,46 @@ class NDConfiguration:
             object.__setattr__(self, "_inline", cached)      # a cache beside the (frozen) fields, not one of them
         return cached
 
+    def asRows(self):
+        """(first element, rows, columns, elements from one row to the next) where the elements of the last axis lie next
+        to each other and the rows -- the leading axes in row-major order -- lie one pitch apart; None for any other view."""
+        if "_rows" not in self.__dict__:
+            object.__setattr__(self, "_rows", None if self.virtual else self._findRows())
+        return self.__dict__["_rows"]
+
+    def _findRows(self):
+        steps = [s * p for s, p in zip(self.strides, self.spread)]
+        base = sum(o * s for o, s in zip(self.offset, self.strides))
+        cols = self.shape[-1]
+        if cols > 1 and steps[-1] != 1:
+            return None
+        rows, pitch = 1, None
+        for extent, step in zip(self.shape[-2::-1], steps[-2::-1]):
+            if extent == 1:
+                continue
+            if pitch is None:
+                pitch = step
+            elif step != pitch * rows:
+                return None
+            rows *= extent
+        pitch = cols if pitch is None else pitch
+        return (base, rows, cols, pitch) if pitch >= cols else None
+
+    def asDense(self):
+        """First element of a view whose elements lie next to each other in row-major order; None for any other view."""
+        rows = self.asRows()
+        return rows[0] if rows is not None and (rows[1] == 1 or rows[3] == rows[2]) else None
+
+    def asDenseColumns(self):
+        """First element of a matrix whose columns lie one behind the other, each contiguous (the transpose of a dense
+        matrix); None for any other view."""
+        if self.virtual or len(self.shape) != 2:
+            return None
+        (rows, cols), steps = self.shape, [s * p for s, p in zip(self.strides, self.spread)]
+        if (rows > 1 and steps[0] != 1) or (cols > 1 and steps[1] != rows):
+            return None
+        return sum(o * s for o, s in zip(self.offset, self.strides))
+
     # ---- derived views ---------------------------------------------------------------------
     def newReshaped(self, newForm: Sequence[int]) -> "NDConfiguration":
         """Permutation / padding view: ``AbstractNDC._simpleReshape`` (AbstractNDC.java:182-203).  For a

@@ -277,6 +277,24 @@ class Tensor:
         from .function import execute
         return execute("dot", [self, b])
 
+    # ---- the operators of a feed-forward sublayer (one kernel each; the reference composes them) ------
+    def layerNorm(self, gain: "Tensor", bias: "Tensor", epsilon: float = 1e-5) -> "Tensor":
+        """(x - mean) / sqrt(variance + epsilon) * gain + bias over the last axis; gain and bias hold one element per column."""
+        from .function import execute
+        return execute("layerNorm", [self, gain, bias], args={"epsilon": float(epsilon)})
+
+    def dropout(self, probability: float, seed: int, offset: int = 0) -> "Tensor":
+        """Every element is dropped with the given probability or divided by 1 - probability.  The choice is a function of
+        (seed, offset) and the element's row-major index: calls that shall draw independently differ in seed or offset."""
+        from .function import execute
+        return execute("dropout", [self], args={"probability": float(probability), "seed": int(seed), "offset": int(offset)})
+
+    def gatedMatMul(self, gate: "Tensor", up: "Tensor", activation: str = "silu") -> "Tensor":
+        """activation(x @ gate) * (x @ up) over the last axis of x; the weights are [K, N], by rows or (as ``T()`` of a dense
+        [N, K]) by columns; activation: idy, relu, sig, silu, gelu or tanh."""
+        from .function import execute
+        return execute("gatedMatMul", [self, gate, up], args={"activation": activation})
+
     def __getattr__(self, name):
         # activation shorthands: t.tanh(), t.sig(), t.relu() ...
         from .backend import ACTIVATIONS
@@ -356,9 +374,10 @@ class GraphNode:
     """What an operation records for reverse-mode AD (autograd/GraphNode.java:121-277): its parents and,
     per parent, the ADAction that turns an error of the result into an error of that parent."""
 
-    def __init__(self, parents: Sequence[Tensor], actions):
+    def __init__(self, parents: Sequence[Tensor], actions, joint=None):
         self.parents = list(parents)
         self.actions = list(actions)         # callables error -> Tensor, or None for non-differentiated parents
+        self.joint = joint                   # instead of the actions: a callable error -> [Tensor or None per parent]
 
 
 def _backward(result: Tensor, error: Tensor) -> None:
@@ -370,6 +389,11 @@ def _backward(result: Tensor, error: Tensor) -> None:
             result.gradient = execute("add", [result.gradient, error], record=False)
     node = result._node
     if node is None:
+        return
+    if node.joint is not None:
+        for parent, parent_error in zip(node.parents, node.joint(error)):
+            if parent_error is not None:
+                _backward(parent, parent_error)
         return
     for parent, action in zip(node.parents, node.actions):
         if action is None:
