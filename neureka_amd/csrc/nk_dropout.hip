@@ -97,6 +97,7 @@ extern "C" int nk_dropout(nk_dev h, int dtype, int rank, nk_buf drn, const int32
     }
     NK_REQUIRE(n == size, "nk_dropout: n = %lld, the drain has %lld elements", (long long)n, (long long)size);
     const int eb = dtype_bytes(dtype);
+    NK_REQUIRE(drn % eb == 0 && src % eb == 0, "nk_dropout: a buffer does not start at an element");
     if (int e = check_extent(dev, "nk_dropout(drn)", drn, drn_cfg, rank, eb)) return e;
     if (int e = check_extent(dev, "nk_dropout(src)", src, src_cfg, rank, eb)) return e;
     Cfg dc, sc;

@@ -180,6 +180,249 @@ __global__ __launch_bounds__(256) void product_kernel(const Product<T> g) {
         }
 }
 
+// ---- f32 products on the bf16 matrix cores ------------------------------------------------------------------------
+// A float is the sum of three bfloat16 numbers, each the rest of the ones before rounded to nearest: 3 x 8 bits hold its 24 (below
+// 2^-110 the last of them leaves bfloat16's range, and the sum is off by at most 2^-134).  Of the nine partial products the
+// six largest are added, x0 y0, x0 y1, x1 y0, x1 y1, x0 y2, x2 y0; the other three are at most 2^-26 of x y each, less than the
+// rounding of an f32 product.  Partial products are exact and their sums are f32, as in a product of floats.  The bf16
+// instruction does 16 times the work of the f32 one per cycle, so six of them cost 6 / 16 of one f32 product.
+//
+// A non-finite operand has no such sum (infinity - infinity), so a wavefront that finds a non-finite result computes its tile
+// once more with the f32 instruction, straight from memory: what comes out is what f32 arithmetic gives.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// two floats -> their three bfloat16 pairs
+__device__ __forceinline__ void split_pair(float x, float y, unsigned (&p)[3]) {
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+        const f32x2 v = {x, y};
+        p[k] = __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+        if (k < 2) {
+            x -= __builtin_bit_cast(float, p[k] << 16);
+            y -= __builtin_bit_cast(float, p[k] & 0xffff0000u);
+        }
+    }
+}
+
+// LDS holds an operand's slice (WIDTH rows x 16 l) as three planes of fragments of 32 rows x 16 l in the order in which the
+// lanes of v_mfma_f32_32x32x16_bf16 take them: lane l gets the 8 values of row l % 32 from 8 (l / 32) on, 16 bytes.  The upper half's
+// rows are rotated by 8 (row ^ 8) so that the writes below do not meet in one bank; a read is 1 KiB without a gap either way.
+template <int WIDTH, bool ALONG, int THREADS>
+struct SplitShare {
+    static constexpr int E = WIDTH * 16 / THREADS;          // elements per thread: 4 or 8
+    static constexpr unsigned PLANE = WIDTH * 32;           // bytes
+    static_assert(E == 4 || E == 8, "a thread moves one or two times four elements");
+    float v[E];
+    const float* base[E / 4];                               // ALONG: the thread's rows; else: its column (base[0])
+    int l_of;                                               // first l of the thread inside a slice
+
+    __device__ __forceinline__ void place(const float* a, int64_t ld, int first, int count, int t, int half_of_columns, const float* other) {
+        // half_of_columns > 0: rows from there on belong to the second matrix of a pair
+#pragma unroll
+        for (int u = 0; u < E / 4; u++) {
+            int r = ALONG ? (t + u * THREADS) >> 2 : t % WIDTH;
+            const float* from = a;
+            if (half_of_columns > 0 && r >= half_of_columns) { r -= half_of_columns; from = other; }
+            const int64_t row = first + r < count ? first + r : count - 1;       // past the end: the last one, its results are not stored
+            base[u] = from + row * (ALONG ? ld : 1);
+        }
+        l_of = ALONG ? (t & 3) * 4 : __builtin_amdgcn_readfirstlane(t / WIDTH) * E;
+    }
+    __device__ __forceinline__ void load(int64_t shift, int64_t ld, int l0, int inner) {      // shift: from the first segment to this one
+        const int l = l0 + l_of;
+        if constexpr (ALONG) {
+            if (l0 + 16 <= inner) {
+#pragma unroll
+                for (int u = 0; u < E / 4; u++) {
+                    const f32x4 q = *(const f32x4_any*)(base[u] + shift + l);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[u * 4 + e] = q[e];
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < E / 4; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[u * 4 + e] = l + e < inner ? base[u][shift + l + e] : 0.0f;
+            }
+        } else {
+            const float* const at = base[0] + shift + (int64_t)l * ld;
+            if (l0 + 16 <= inner) {
+#pragma unroll
+                for (int e = 0; e < E; e++) v[e] = at[(int64_t)e * ld];
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++) v[e] = l + e < inner ? at[(int64_t)e * ld] : 0.0f;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(unsigned char* lds, int t) const {
+        unsigned p[E / 2][3];
+#pragma unroll
+        for (int e = 0; e < E / 2; e++) split_pair(v[2 * e], v[2 * e + 1], p[e]);
+        if constexpr (ALONG) {
+            const int q = t & 3, high = q >> 1;
+#pragma unroll
+            for (int u = 0; u < E / 4; u++) {
+                const int r = (t + u * THREADS) >> 2;
+                unsigned char* const at = lds + (r >> 5) * 1024 + high * 512 + ((r & 31) ^ (high * 8)) * 16 + (q & 1) * 8;
+#pragma unroll
+                for (int k = 0; k < 3; k++) *(uint2*)(at + k * PLANE) = make_uint2(p[u * 2][k], p[u * 2 + 1][k]);
+            }
+        } else {
+            const int r = t % WIDTH, l = l_of, high = l >> 3;
+            unsigned char* const at = lds + (r >> 5) * 1024 + high * 512 + ((r & 31) ^ (high * 8)) * 16 + (l & 4) * 2;
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+                if constexpr (E == 8) *(uint4*)(at + k * PLANE) = make_uint4(p[0][k], p[1][k], p[2][k], p[3][k]);
+                else                  *(uint2*)(at + k * PLANE) = make_uint2(p[0][k], p[1][k]);
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ void lds_barrier() {             // orders LDS only: requests to memory stay in flight
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// WM x WN wavefronts, each with a tile of FI x FJ fragments of 32 x 32.  PAIRED: the first half of a wavefront's column
+// fragments comes from the first product, the second half from the second.
+template <int WM, int WN, int FI, int FJ, bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
+__global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Product<float> g) {
+    constexpr int THREADS = WM * WN * 64, BM = WM * FI * 32, BN = WN * FJ * 32, HALF = PAIRED ? BN / 2 : BN;
+    typedef SplitShare<BM, A_ALONG, THREADS> AShare;
+    typedef SplitShare<BN, B_ALONG, THREADS> BShare;
+    constexpr unsigned A_BYTES = 3 * AShare::PLANE, BUFFER = A_BYTES + 3 * BShare::PLANE;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];          // two buffers
+    const unsigned tiles = (unsigned)(g.tiles_m * g.tiles_n), part = blockIdx.x / tiles;
+    int tm, tn;
+    own_tile(blockIdx.x - part * tiles, tiles, g.tiles_m, g.tiles_n, tm, tn);
+    const int m0 = tm * BM, n0 = tn * HALF;
+    const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, wm = wave / WN, wn = wave % WN;
+    AShare a;
+    BShare b;
+    a.place(g.A[0], g.lda, m0, g.rows, t, 0, nullptr);
+    b.place(g.B[0], g.ldb, n0, g.cols, t, PAIRED ? HALF : 0, g.B[1]);
+    const int64_t a_shift = g.segments > 1 ? g.A[1] - g.A[0] : 0, b_shift = g.segments > 1 ? g.B[1] - g.B[0] : 0;
+    const int per_segment = (g.inner + 15) / 16;
+    const int first = (int)part * g.steps_per_part, all = per_segment * g.segments;
+    const int last = first + g.steps_per_part < all ? first + g.steps_per_part : all;
+    const auto request_a = [&](int s) {
+        const int segment = s >= per_segment;
+        a.load(segment ? a_shift : 0, g.lda, (s - segment * per_segment) * 16, g.inner);
+    };
+    const auto request_b = [&](int s) {
+        const int segment = s >= per_segment;
+        b.load(segment ? b_shift : 0, g.ldb, (s - segment * per_segment) * 16, g.inner);
+    };
+    const auto column_block = [&](int j) { return PAIRED ? (j / (FJ / 2)) * (BN / 64) + wn * (FJ / 2) + j % (FJ / 2) : wn * FJ + j; };
+    const unsigned mine = (unsigned)((lane >> 5) * 512 + (((lane & 31) ^ ((lane >> 5) * 8)) * 16));
+    f32x16 acc[FI][FJ] = {};
+
+    request_a(first); request_b(first);
+    a.store(lds, t); b.store(lds + A_BYTES, t);
+    if (first + 1 < last) { request_a(first + 1); request_b(first + 1); }
+    lds_barrier();
+    for (int s = first; s < last; s++) {
+        const unsigned char* const cur = lds + ((s - first) & 1) * BUFFER + mine;
+        unsigned char* const next = lds + ((s - first + 1) & 1) * BUFFER;
+        bf16x8 bf[FJ][3];
+#pragma unroll
+        for (int j = 0; j < FJ; j++)
+#pragma unroll
+            for (int k = 0; k < 3; k++) bf[j][k] = *(const bf16x8*)(cur + A_BYTES + k * BShare::PLANE + column_block(j) * 1024);
+#pragma unroll
+        for (int i = 0; i < FI; i++) {
+            bf16x8 af[3];
+#pragma unroll
+            for (int k = 0; k < 3; k++) af[k] = *(const bf16x8*)(cur + k * AShare::PLANE + (wm * FI + i) * 1024);
+            constexpr int order[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
+#pragma unroll
+            for (int c = 0; c < 6; c++)
+#pragma unroll
+                for (int j = 0; j < FJ; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[order[c][0]], bf[j][order[c][1]], acc[i][j], 0, 0, 0);
+            // the next slice's operands go to LDS between the matrix instructions; their registers take the slice after it
+            if (i == 0 && s + 1 < last) {
+                a.store(next, t);
+                if (s + 2 < last) request_a(s + 2);
+            }
+            if (i == FI / 2 && s + 1 < last) {
+                b.store(next + A_BYTES, t);
+                if (s + 2 < last) request_b(s + 2);
+            }
+        }
+        lds_barrier();
+    }
+
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < FI; i++)
+#pragma unroll
+        for (int j = 0; j < FJ; j++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) odd |= !(__builtin_fabsf(acc[i][j][v]) < INFINITY);
+    // one fragment of the result (PAIRED: the same fragment of both products) to where it belongs.
+    // Register v of lane l: row 8 (v / 4) + 4 (l / 32) + v % 4, column l % 32 of the fragment.
+    const int64_t shift = (int64_t)part * g.part_stride;
+    const auto write = [&](int i, int j, const f32x16& x, const f32x16& y) {
+        const int n = n0 + (PAIRED ? wn * (FJ / 2) + j : wn * FJ + j) * 32 + (lane & 31);
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+            const int m = m0 + (wm * FI + i) * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
+            if (m >= g.rows || n >= g.cols) continue;
+            const int64_t at = (int64_t)m * g.cols + n + shift;
+            if constexpr (PAIRED && EPI == GATED) {
+                g.out[0][at] = gated_fun(g.fun, x[v]) * y[v];
+                if (g.out[1]) { g.out[1][at] = x[v]; g.out[2][at] = y[v]; }
+            } else {
+                g.out[0][at] = x[v];
+                if constexpr (PAIRED) g.out[1][at] = y[v];
+            }
+        }
+    };
+    constexpr int SHOWN = PAIRED ? FJ / 2 : FJ;             // fragments per row of the wavefront's tile, of one product
+    if (!__any(odd)) {
+#pragma unroll
+        for (int i = 0; i < FI; i++)
+#pragma unroll
+            for (int j = 0; j < SHOWN; j++) write(i, j, acc[i][j], acc[i][PAIRED ? FJ / 2 + j : j]);
+        return;
+    }
+#pragma unroll 1
+    for (int f = 0; f < FI * SHOWN; f++) {
+        const int i = f / SHOWN, j = f % SHOWN;
+        const int m = m0 + (wm * FI + i) * 32 + (lane & 31), n = n0 + (PAIRED ? wn * (FJ / 2) + j : wn * FJ + j) * 32 + (lane & 31);
+        const int64_t am = (int64_t)(m < g.rows ? m : g.rows - 1) * (A_ALONG ? g.lda : 1), bn = (int64_t)(n < g.cols ? n : g.cols - 1) * (B_ALONG ? g.ldb : 1);
+        f32x16 x = {}, y = {};
+#pragma unroll 1
+        for (int s = first; s < last; s++) {
+            const int segment = s >= per_segment, l0 = (s - segment * per_segment) * 16;
+            const float* const ap = g.A[segment] + am;
+            const float* const bp = g.B[PAIRED ? 0 : segment] + bn;
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+                const int l = l0 + k + (lane >> 5);
+                const bool in = l < g.inner;
+                const int64_t ao = (int64_t)(in ? l : 0) * (A_ALONG ? 1 : g.lda), bo = (int64_t)(in ? l : 0) * (B_ALONG ? 1 : g.ldb);
+                const float av = in ? ap[ao] : 0.0f, bv = in ? bp[bo] : 0.0f;
+                x = __builtin_amdgcn_mfma_f32_32x32x2f32(av, bv, x, 0, 0, 0);
+                if constexpr (PAIRED) {
+                    const float cv = in ? g.B[1][bn + bo] : 0.0f;
+                    y = __builtin_amdgcn_mfma_f32_32x32x2f32(av, cv, y, 0, 0, 0);
+                }
+            }
+        }
+        write(i, j, x, y);
+    }
+}
+
 // ---- parts of the contraction, added in order -----------------------------------------------------------------------
 // partial: [parts][halves][n]; halves 2: the pair of products
 template <typename T, bool PAIRED, int EPI>
@@ -214,12 +457,18 @@ __global__ __launch_bounds__(256) void gated_errors_kernel(int fun, int64_t n, c
 }
 
 // ---- plans ---------------------------------------------------------------------------------------------------------------
-struct Split { int tiles_m, tiles_n, parts, steps_per_part; };
+struct Split { bool large; int tiles_m, tiles_n, parts, steps_per_part; };
+template <typename T>
 static Split plan(const Device* dev, bool paired, int64_t rows, int64_t cols, int64_t inner, int segments) {
     Split s;
-    s.tiles_m = (int)((rows + 127) / 128);
-    s.tiles_n = (int)(paired ? (cols + 63) / 64 : (cols + 127) / 128);
-    const int64_t tiles = (int64_t)s.tiles_m * s.tiles_n, steps = (inner + 15) / 16 * segments, want = 2 * dev->props.multiProcessorCount;
+    const int64_t cus = dev->props.multiProcessorCount, steps = (inner + 15) / 16 * segments;
+    const auto tile = [&](int64_t edge) {
+        s.tiles_m = (int)((rows + edge - 1) / edge);
+        s.tiles_n = (int)(paired ? (cols + edge / 2 - 1) / (edge / 2) : (cols + edge - 1) / edge);
+        return (int64_t)s.tiles_m * s.tiles_n;
+    };
+    s.large = sizeof(T) == 4 && tile(256) >= cus;
+    const int64_t tiles = tile(s.large ? 256 : 128), want = (s.large ? 1 : 2) * cus;
     int64_t parts = tiles >= want ? 1 : want / tiles;
     if (parts > steps / 8) parts = steps / 8 > 0 ? steps / 8 : 1;
     s.steps_per_part = (int)((steps + parts - 1) / parts);
@@ -230,6 +479,20 @@ static uint64_t partial_elements(const Split& s, bool paired, int64_t rows, int6
     return s.parts > 1 ? (uint64_t)s.parts * (paired ? 2 : 1) * rows * cols : 0;
 }
 
+template <bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
+static void launch_tiles(Device* dev, const Product<float>& g, const Split& s, dim3 grid) {
+    const auto go = [&](auto kernel, int threads, unsigned lds) {
+        (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, dev->stream, g);
+    };
+    if (s.large) go(split_product_kernel<2, 4, 4, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 512, 2 * 2 * 3 * 256 * 32);
+    else         go(split_product_kernel<2, 2, 2, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 256, 2 * 2 * 3 * 128 * 32);
+}
+template <bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
+static void launch_tiles(Device* dev, const Product<double>& g, const Split&, dim3 grid) {
+    hipLaunchKernelGGL((product_kernel<double, A_ALONG, B_ALONG, PAIRED, EPI>), grid, dim3(256), 0, dev->stream, g);
+}
+
 template <typename T, bool PAIRED, int EPI>
 static void launch_product(Device* dev, Product<T> g, const Split& s, bool a_along, bool b_along, T* partial) {
     g.tiles_m = s.tiles_m; g.tiles_n = s.tiles_n; g.steps_per_part = s.steps_per_part;
@@ -238,9 +501,10 @@ static void launch_product(Device* dev, Product<T> g, const Split& s, bool a_alo
     const dim3 grid((unsigned)(s.tiles_m * s.tiles_n * s.parts));
     const auto go = [&](auto epi) {
         constexpr int E = decltype(epi)::value;
-        if (a_along && b_along)       hipLaunchKernelGGL((product_kernel<T, true, true, PAIRED, E>), grid, dim3(256), 0, dev->stream, g);
-        else if (a_along)             hipLaunchKernelGGL((product_kernel<T, true, false, PAIRED, E>), grid, dim3(256), 0, dev->stream, g);
-        else                          hipLaunchKernelGGL((product_kernel<T, false, false, PAIRED, E>), grid, dim3(256), 0, dev->stream, g);
+        // (a transposed input only in the pair of weight gradients, where the errors lie by rows)
+        if constexpr (PAIRED && E == STORE) { if (!a_along) { launch_tiles<false, false, PAIRED, E>(dev, g, s, grid); return; } }
+        if (b_along) launch_tiles<true, true, PAIRED, E>(dev, g, s, grid);
+        else         launch_tiles<true, false, PAIRED, E>(dev, g, s, grid);
     };
     if (s.parts == 1) { go(std::integral_constant<int, EPI>()); return; }
     g.out[0] = partial; g.out[1] = partial + n; g.out[2] = nullptr;
@@ -255,7 +519,7 @@ static int gated_forward(Device* dev, int fun, bool along, int64_t M, int64_t K,
     g.A[0] = X; g.lda = K; g.B[0] = Wg; g.B[1] = Wu; g.ldb = along ? K : N;
     g.rows = (int)M; g.cols = (int)N; g.inner = (int)K; g.segments = 1; g.fun = fun;
     g.out[0] = H; g.out[1] = gate; g.out[2] = up;
-    const Split s = plan(dev, true, M, N, K, 1);
+    const Split s = plan<T>(dev, true, M, N, K, 1);
     void* ws = nullptr;
     if (const uint64_t need = partial_elements(s, true, M, N))
         if (int e = workspace(dev, need * sizeof(T), &ws)) return e;
@@ -269,7 +533,7 @@ template <typename T>
 static int gated_backward(Device* dev, int fun, bool along, int64_t M, int64_t K, int64_t N, const T* X, const T* Wg, const T* Wu, const T* gate, const T* up,
                           const T* E, T* dX, T* dWg, T* dWu) {
     const int64_t n = M * N;
-    const Split sx = plan(dev, false, M, K, N, 2), sw = plan(dev, true, K, N, M, 1);
+    const Split sx = plan<T>(dev, false, M, K, N, 2), sw = plan<T>(dev, true, K, N, M, 1);
     const uint64_t px = dX ? partial_elements(sx, false, M, K) : 0, pw = dWg ? partial_elements(sw, true, K, N) : 0;
     void* ws = nullptr;
     if (int e = workspace(dev, (2 * (uint64_t)n + (px > pw ? px : pw)) * sizeof(T), &ws)) return e;
@@ -306,9 +570,10 @@ static int check_gated(const char* what, int fun, int dtype, int layout, int64_t
 }
 struct Piece { const char* name; nk_buf at; uint64_t bytes; };
 // every piece inside a live buffer, and no output (the last `outputs` pieces) on another piece
-static int check_pieces(Device* dev, const char* what, const Piece* p, int count, int outputs) {
+static int check_pieces(Device* dev, const char* what, const Piece* p, int count, int outputs, uint64_t element) {
     for (int i = 0; i < count; i++) {
         if (!p[i].at && i >= count - outputs) continue;
+        NK_REQUIRE(p[i].at % element == 0, "%s: %s does not start at an element", what, p[i].name);
         if (int e = check_range(dev, p[i].name, p[i].at, 0, p[i].bytes)) return e;
     }
     for (int i = count - outputs; i < count; i++)
@@ -330,7 +595,7 @@ extern "C" int nk_gated_matmul(nk_dev h, int fun, int dtype, int layout, int64_t
     NK_REQUIRE((gate == 0) == (up == 0), "%s: gate and up are kept together or not at all", what);
     const uint64_t eb = dtype_bytes(dtype), x = M * K * eb, w = K * N * eb, y = M * N * eb;
     const Piece p[] = {{"X", X, x}, {"Wg", Wg, w}, {"Wu", Wu, w}, {"the drain", drn, y}, {"gate", gate, y}, {"up", up, y}};
-    if (int e = check_pieces(dev, what, p, 6, 3)) return e;
+    if (int e = check_pieces(dev, what, p, 6, 3, eb)) return e;
     const bool along = layout == NK_LAYOUT_COLUMN_MAJOR;
     return dtype == NK_F32 ? gated_forward<float>(dev, fun, along, M, K, N, (const float*)X, (const float*)Wg, (const float*)Wu, (float*)drn, (float*)gate, (float*)up)
                            : gated_forward<double>(dev, fun, along, M, K, N, (const double*)X, (const double*)Wg, (const double*)Wu, (double*)drn, (double*)gate, (double*)up);
@@ -345,7 +610,7 @@ extern "C" int nk_gated_matmul_backward(nk_dev h, int fun, int dtype, int layout
     NK_REQUIRE((dWg == 0) == (dWu == 0), "%s: the gradients of the weights are computed together or not at all", what);
     const uint64_t eb = dtype_bytes(dtype), x = M * K * eb, w = K * N * eb, y = M * N * eb;
     const Piece p[] = {{"X", X, x}, {"Wg", Wg, w}, {"Wu", Wu, w}, {"gate", gate, y}, {"up", up, y}, {"error", error, y}, {"d_X", dX, x}, {"d_Wg", dWg, w}, {"d_Wu", dWu, w}};
-    if (int e = check_pieces(dev, what, p, 9, 3)) return e;
+    if (int e = check_pieces(dev, what, p, 9, 3, eb)) return e;
     const bool along = layout == NK_LAYOUT_COLUMN_MAJOR;
     return dtype == NK_F32 ? gated_backward<float>(dev, fun, along, M, K, N, (const float*)X, (const float*)Wg, (const float*)Wu, (const float*)gate, (const float*)up,
                                                    (const float*)error, (float*)dX, (float*)dWg, (float*)dWu)

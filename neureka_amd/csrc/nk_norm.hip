@@ -409,6 +409,7 @@ extern "C" int nk_layer_norm(nk_dev h, int dtype, int64_t rows, int64_t cols, nk
         if (int e = check_range(dev, "nk_layer_norm(mean)", mean, 0, rows * eb)) return e;
         if (int e = check_range(dev, "nk_layer_norm(rstd)", rstd, 0, rows * eb)) return e;
     }
+    for (nk_buf b : {src, gain, bias, drn, mean, rstd}) NK_REQUIRE(b % eb == 0, "%s: a buffer does not start at an element", what);
     const nk_buf outs[3] = {drn, mean, rstd};
     const uint64_t lens[3] = {size, rows * eb, rows * eb};
     for (int i = 0; i < 3; i++) {
@@ -439,6 +440,7 @@ extern "C" int nk_layer_norm_backward(nk_dev h, int dtype, int64_t rows, int64_t
     const char* const in_names[5] = {"nk_layer_norm_backward(src)", "nk_layer_norm_backward(gain)", "nk_layer_norm_backward(mean)",
                                      "nk_layer_norm_backward(rstd)", "nk_layer_norm_backward(error)"};
     const char* const out_names[3] = {"nk_layer_norm_backward(d_src)", "nk_layer_norm_backward(d_gain)", "nk_layer_norm_backward(d_bias)"};
+    for (nk_buf b : {src, gain, mean, rstd, error, d_src, d_gain, d_bias}) NK_REQUIRE(b % eb == 0, "%s: a buffer does not start at an element", what);
     for (int i = 0; i < 5; i++)
         if (int e = check_range(dev, in_names[i], ins[i], 0, in_lens[i])) return e;
     for (int i = 0; i < 3; i++) {
