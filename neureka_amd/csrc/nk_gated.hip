@@ -233,31 +233,27 @@ struct SplitShare {
         }
         l_of = ALONG ? (t & 3) * 4 : __builtin_amdgcn_readfirstlane(t / WIDTH) * E;
     }
-    __device__ __forceinline__ void load(int64_t shift, int64_t ld, int l0, int inner) {      // shift: from the first segment to this one
+    // shift: from the first segment to this one.  WHOLE: all 16 l of the slice exist; else what lies past `inner` is zero.
+    template <bool WHOLE>
+    __device__ __forceinline__ void load(int64_t shift, int64_t ld, int l0, int inner) {
         const int l = l0 + l_of;
         if constexpr (ALONG) {
-            if (l0 + 16 <= inner) {
 #pragma unroll
-                for (int u = 0; u < E / 4; u++) {
-                    const f32x4 q = *(const f32x4_any*)(base[u] + shift + l);
+            for (int u = 0; u < E / 4; u++) {
+                const float* const at = base[u] + shift + l;
+                if constexpr (WHOLE) {
+                    const f32x4 q = *(const f32x4_any*)at;
 #pragma unroll
                     for (int e = 0; e < 4; e++) v[u * 4 + e] = q[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[u * 4 + e] = l + e < inner ? at[e] : 0.0f;
                 }
-            } else {
-#pragma unroll
-                for (int u = 0; u < E / 4; u++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[u * 4 + e] = l + e < inner ? base[u][shift + l + e] : 0.0f;
             }
         } else {
             const float* const at = base[0] + shift + (int64_t)l * ld;
-            if (l0 + 16 <= inner) {
 #pragma unroll
-                for (int e = 0; e < E; e++) v[e] = at[(int64_t)e * ld];
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; e++) v[e] = l + e < inner ? at[(int64_t)e * ld] : 0.0f;
-            }
+            for (int e = 0; e < E; e++) v[e] = WHOLE || l + e < inner ? at[(int64_t)e * ld] : 0.0f;
         }
     }
     __device__ __forceinline__ void store(unsigned char* lds, int t) const {
@@ -310,55 +306,111 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
     a.place(g.A[0], g.lda, m0, g.rows, t, 0, nullptr);
     b.place(g.B[0], g.ldb, n0, g.cols, t, PAIRED ? HALF : 0, g.B[1]);
     const int64_t a_shift = g.segments > 1 ? g.A[1] - g.A[0] : 0, b_shift = g.segments > 1 ? g.B[1] - g.B[0] : 0;
-    const int per_segment = (g.inner + 15) / 16;
-    const int first = (int)part * g.steps_per_part, all = per_segment * g.segments;
+    // Whole slices of all segments first, g.steps_per_part of them per part; the last part also takes what is left of each segment.
+    const int whole = g.inner / 16, all = whole * g.segments;
+    const int first = (int)part * g.steps_per_part < all ? (int)part * g.steps_per_part : all;
     const int last = first + g.steps_per_part < all ? first + g.steps_per_part : all;
     const auto request_a = [&](int s) {
-        const int segment = s >= per_segment;
-        a.load(segment ? a_shift : 0, g.lda, (s - segment * per_segment) * 16, g.inner);
+        const int segment = s >= whole;
+        a.template load<true>(segment ? a_shift : 0, g.lda, (s - segment * whole) * 16, g.inner);
     };
     const auto request_b = [&](int s) {
-        const int segment = s >= per_segment;
-        b.load(segment ? b_shift : 0, g.ldb, (s - segment * per_segment) * 16, g.inner);
+        const int segment = s >= whole;
+        b.template load<true>(segment ? b_shift : 0, g.ldb, (s - segment * whole) * 16, g.inner);
     };
     const auto column_block = [&](int j) { return PAIRED ? (j / (FJ / 2)) * (BN / 64) + wn * (FJ / 2) + j % (FJ / 2) : wn * FJ + j; };
     const unsigned mine = (unsigned)((lane >> 5) * 512 + (((lane & 31) ^ ((lane >> 5) * 8)) * 16));
     f32x16 acc[FI][FJ] = {};
+    const auto read_a = [&](const unsigned char* from, int i, bf16x8 (&f)[3]) {
+#pragma unroll
+        for (int k = 0; k < 3; k++) f[k] = *(const bf16x8*)(from + mine + k * AShare::PLANE + (wm * FI + i) * 1024);
+    };
+    const auto read_b = [&](const unsigned char* from, bf16x8 (&f)[FJ][3]) {
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+#pragma unroll
+            for (int j = 0; j < FJ; j++) f[j][k] = *(const bf16x8*)(from + mine + A_BYTES + k * BShare::PLANE + column_block(j) * 1024);
+    };
+    const auto multiply = [&](int i, const bf16x8 (&af)[3], const bf16x8 (&bf)[FJ][3]) {
+        constexpr int order[6][2] = {{0, 0}, {1, 0}, {2, 0}, {0, 1}, {1, 1}, {0, 2}};
+#pragma unroll
+        for (int c = 0; c < 6; c++)
+#pragma unroll
+            for (int j = 0; j < FJ; j++)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[order[c][0]], bf[j][order[c][1]], acc[i][j], 0, 0, 0);
+    };
 
-    request_a(first); request_b(first);
-    a.store(lds, t); b.store(lds + A_BYTES, t);
-    if (first + 1 < last) { request_a(first + 1); request_b(first + 1); }
-    lds_barrier();
-    for (int s = first; s < last; s++) {
-        const unsigned char* const cur = lds + ((s - first) & 1) * BUFFER + mine;
-        unsigned char* const next = lds + ((s - first + 1) & 1) * BUFFER;
-        bf16x8 bf[FJ][3];
+    if (first < last) {
+        // The loop is one block without a branch.  Slice s is in LDS and the first fragments of it in registers; slice s + 1 is in
+        // registers as floats and goes to LDS between the matrix instructions, slice s + 2 is requested as soon as its registers are
+        // free (past the end: the last slice once more).  The barrier stands before the last row of fragments: behind it, while those
+        // are multiplied, the first fragments of the next slice are read.
+        const auto clamp = [&](int s) { return s < last ? s : last - 1; };
+        request_a(first); request_b(first);
+        a.store(lds, t); b.store(lds + A_BYTES, t);
+        request_a(clamp(first + 1)); request_b(clamp(first + 1));
+        lds_barrier();
+        bf16x8 bf[FJ][3], af[2][3];
+        read_b(lds, bf);
+        read_a(lds, 0, af[0]);
+        unsigned now = 0;
+        for (int s = first; s < last; s++) {
+            const unsigned char* const cur = lds + now;
+            unsigned char* const next = lds + (BUFFER - now);
 #pragma unroll
-        for (int j = 0; j < FJ; j++)
+            for (int i = 0; i < FI - 1; i++) {
+                read_a(cur, i + 1, af[(i + 1) & 1]);
+                multiply(i, af[i & 1], bf);
+                if (i == 0) { a.store(next, t); request_a(clamp(s + 2)); }
+                if (i == (FI > 2 ? 1 : 0)) { b.store(next + A_BYTES, t); request_b(clamp(s + 2)); }
 #pragma unroll
-            for (int k = 0; k < 3; k++) bf[j][k] = *(const bf16x8*)(cur + A_BYTES + k * BShare::PLANE + column_block(j) * 1024);
-#pragma unroll
-        for (int i = 0; i < FI; i++) {
-            bf16x8 af[3];
-#pragma unroll
-            for (int k = 0; k < 3; k++) af[k] = *(const bf16x8*)(cur + k * AShare::PLANE + (wm * FI + i) * 1024);
-            constexpr int order[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
-#pragma unroll
-            for (int c = 0; c < 6; c++)
-#pragma unroll
-                for (int j = 0; j < FJ; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[order[c][0]], bf[j][order[c][1]], acc[i][j], 0, 0, 0);
-            // the next slice's operands go to LDS between the matrix instructions; their registers take the slice after it
-            if (i == 0 && s + 1 < last) {
-                a.store(next, t);
-                if (s + 2 < last) request_a(s + 2);
+                for (int n = 0; n < 6 * FJ; n++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);           // a matrix instruction,
+                    __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);           // vector arithmetic in its shadow,
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);           // an LDS read,
+                    __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);           // an LDS write,
+                    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);           // a request to memory
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (i == FI / 2 && s + 1 < last) {
-                b.store(next + A_BYTES, t);
-                if (s + 2 < last) request_b(s + 2);
+            lds_barrier();
+            bf16x8 bn[FJ][3], an[3];
+            read_a(next, 0, an);
+            read_b(next, bn);
+            multiply(FI - 1, af[(FI - 1) & 1], bf);
+#pragma unroll
+            for (int n = 0; n < 3 + 3 * FJ; n++) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
+            // (without the empty statements the compiler moves these reads to the head of the loop, where nothing hides them)
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+                asm volatile("" : "+v"(an[k]));
+                af[0][k] = an[k];
+#pragma unroll
+                for (int j = 0; j < FJ; j++) {
+                    asm volatile("" : "+v"(bn[j][k]));
+                    bf[j][k] = bn[j][k];
+                }
+            }
+            now = BUFFER - now;
         }
         lds_barrier();
+    }
+    if (g.inner % 16 != 0 && last == all) {
+        for (int segment = 0; segment < g.segments; segment++) {
+            a.template load<false>(segment ? a_shift : 0, g.lda, whole * 16, g.inner);
+            b.template load<false>(segment ? b_shift : 0, g.ldb, whole * 16, g.inner);
+            a.store(lds, t); b.store(lds + A_BYTES, t);
+            lds_barrier();
+            bf16x8 bf[FJ][3], af[3];
+            read_b(lds, bf);
+#pragma unroll
+            for (int i = 0; i < FI; i++) { read_a(lds, i, af); multiply(i, af, bf); }
+            lds_barrier();
+        }
     }
 
     bool odd = false;
@@ -401,9 +453,11 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
         const int m = m0 + (wm * FI + i) * 32 + (lane & 31), n = n0 + (PAIRED ? wn * (FJ / 2) + j : wn * FJ + j) * 32 + (lane & 31);
         const int64_t am = (int64_t)(m < g.rows ? m : g.rows - 1) * (A_ALONG ? g.lda : 1), bn = (int64_t)(n < g.cols ? n : g.cols - 1) * (B_ALONG ? g.ldb : 1);
         f32x16 x = {}, y = {};
+        const int turns = last - first + (last == all && g.inner % 16 != 0 ? g.segments : 0);
 #pragma unroll 1
-        for (int s = first; s < last; s++) {
-            const int segment = s >= per_segment, l0 = (s - segment * per_segment) * 16;
+        for (int turn = 0; turn < turns; turn++) {
+            const int s = first + turn, left = s - all;
+            const int segment = left >= 0 ? left : s >= whole, l0 = (left >= 0 ? whole : s - segment * whole) * 16;
             const float* const ap = g.A[segment] + am;
             const float* const bp = g.B[PAIRED ? 0 : segment] + bn;
 #pragma unroll
@@ -461,7 +515,7 @@ struct Split { bool large; int tiles_m, tiles_n, parts, steps_per_part; };
 template <typename T>
 static Split plan(const Device* dev, bool paired, int64_t rows, int64_t cols, int64_t inner, int segments) {
     Split s;
-    const int64_t cus = dev->props.multiProcessorCount, steps = (inner + 15) / 16 * segments;
+    const int64_t cus = dev->props.multiProcessorCount, steps = (sizeof(T) == 4 ? inner / 16 : (inner + 15) / 16) * segments;      // (f32: whole slices)
     const auto tile = [&](int64_t edge) {
         s.tiles_m = (int)((rows + edge - 1) / edge);
         s.tiles_n = (int)(paired ? (cols + edge / 2 - 1) / (edge / 2) : (cols + edge - 1) / edge);
@@ -472,7 +526,9 @@ static Split plan(const Device* dev, bool paired, int64_t rows, int64_t cols, in
     int64_t parts = tiles >= want ? 1 : want / tiles;
     if (parts > steps / 8) parts = steps / 8 > 0 ? steps / 8 : 1;
     s.steps_per_part = (int)((steps + parts - 1) / parts);
+    if (s.steps_per_part < 1) s.steps_per_part = 1;          // (fewer than 16 l)
     s.parts = (int)((steps + s.steps_per_part - 1) / s.steps_per_part);
+    if (s.parts < 1) s.parts = 1;
     return s;
 }
 static uint64_t partial_elements(const Split& s, bool paired, int64_t rows, int64_t cols) {
