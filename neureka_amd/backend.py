@@ -94,10 +94,16 @@ def _new_output(device: HipDevice, dtype, shape, layout: Layout = Layout.ROW_MAJ
     element.  ``overwritten=True`` says that the implementation the drain goes to does exactly that, so the zeros
     would never be read and the fill (a second pass over the output, as long as the kernel itself for a broadcast)
     is left out; the result is the same bit for bit.  Drains a kernel adds to, or writes in part, keep the fill."""
-    from .tensor import Tensor
-    t = Tensor._on_device(device, dtype, shape, layout, zeroed=not overwritten)
+    global _tensor_on_device
+    if _tensor_on_device is None:               # (tensor.py imports this module)
+        from .tensor import Tensor
+        _tensor_on_device = Tensor._on_device
+    t = _tensor_on_device(device, dtype, shape, layout, zeroed=not overwritten)
     t._intermediate = True
     return t
+
+
+_tensor_on_device = None
 
 
 class BiElementwise(Algorithm):
@@ -374,20 +380,21 @@ class DotProductAlgorithm(Algorithm):
 
 
 def _one_type(what: str, tensors) -> None:
-    if any(t.dtype != tensors[0].dtype for t in tensors):
+    first = tensors[0].dtype
+    if not all([t.dtype == first for t in tensors]):
         raise IllegalArgumentException(f"the operands of {what} are of one type, got {', '.join(str(t.dtype) for t in tensors)}")
 
 
 def as_rows(t):
     """The tensor itself where its last axis is contiguous and its rows lie one pitch apart, else a dense copy."""
-    if t.isVirtual():
+    if t._virtual:
         t.setIsVirtual(False)
     return t if t.ndc.asRows() is not None else t.deepCopy()
 
 
 def as_dense(t):
     """The tensor itself where its elements lie next to each other in row-major order, else a dense copy."""
-    if t.isVirtual():
+    if t._virtual:
         t.setIsVirtual(False)
     return t if t.ndc.asDense() is not None else t.deepCopy()
 
@@ -403,17 +410,18 @@ class LayerNormAlgorithm(Algorithm):
     def prepare(self, call):
         src, gain, bias = call.inputs
         _one_type("layerNorm", call.inputs)
-        cols = src.shape[-1]
+        cols = src.ndc.shape[-1]
         for what, t in (("gain", gain), ("bias", bias)):
-            if t.shape[-1] != cols or t.size != cols:
+            if t.ndc.shape[-1] != cols or t.ndc.size != cols:
                 raise IllegalArgumentException(f"the {what} of layerNorm has shape {list(t.shape)}, the last axis of the source {cols} elements")
         if not 0 <= call.args["epsilon"] < float("inf"):
             raise IllegalArgumentException(f"the epsilon of layerNorm is finite and not negative, not {call.args['epsilon']}")
-        src, gain, bias = as_rows(src), as_dense(gain), as_dense(bias)
-        if call.args.get("keep"):
-            rows = src.size // cols
-            call.args["mean"], call.args["rstd"] = (call.device.allocate(src.dtype, rows) for _ in range(2))
-        return call.withInputs([_new_output(call.device, src.dtype, src.shape, overwritten=True), src, gain, bias])
+        src = as_rows(src)
+        if call.args["keep"]:
+            rows = src.ndc.size // cols
+            call.args["mean"], call.args["rstd"] = call.device.allocate(src.dtype, rows), call.device.allocate(src.dtype, rows)
+        call.inputs = [_new_output(call.device, src.dtype, src.ndc.shape, overwritten=True), src, as_dense(gain), as_dense(bias)]
+        return call
 
 
 class DropoutAlgorithm(Algorithm):
@@ -430,8 +438,11 @@ class DropoutAlgorithm(Algorithm):
         for what in ("seed", "offset"):
             if not 0 <= a[what] < 1 << 64:
                 raise IllegalArgumentException(f"the {what} of a dropout is an unsigned 64-bit number, not {a[what]}")
-        src = call.input(0)
-        return call.withInputs([_new_output(call.device, src.dtype, src.shape, overwritten=True), src])
+        src = call.inputs[0]
+        if src._virtual:
+            src.setIsVirtual(False)
+        call.inputs = [_new_output(call.device, src.dtype, src.ndc.shape, overwritten=True), src]
+        return call
 
 
 class GatedMatMulAlgorithm(Algorithm):
@@ -447,20 +458,23 @@ class GatedMatMulAlgorithm(Algorithm):
         _one_type("gatedMatMul", call.inputs)
         if call.args["activation"] not in HipDevice.GATED_ACTIVATIONS:
             raise IllegalArgumentException(f"gatedMatMul takes one of {', '.join(HipDevice.GATED_ACTIVATIONS)}, not '{call.args['activation']}'")
-        if gate.rank != 2 or gate.shape != up.shape or gate.shape[0] != x.shape[-1]:
-            raise IllegalArgumentException(f"weights {list(gate.shape)} and {list(up.shape)} do not fit rows of {x.shape[-1]}: both are [{x.shape[-1]}, columns]")
+        K = x.ndc.shape[-1]
+        if gate.rank != 2 or gate.ndc.shape != up.ndc.shape or gate.ndc.shape[0] != K:
+            raise IllegalArgumentException(f"weights {list(gate.shape)} and {list(up.shape)} do not fit rows of {K}: both are [{K}, columns]")
         x = as_dense(x)
         for w in (gate, up):
-            if w.isVirtual():
+            if w._virtual:
                 w.setIsVirtual(False)
         # both as they lie, by rows or by columns; anything else becomes dense rows
-        if not (all(w.ndc.asDense() is not None for w in (gate, up)) or all(w.ndc.asDenseColumns() is not None for w in (gate, up))):
-            gate, up = as_dense(gate), as_dense(up)
-        shape = x.shape[:-1] + (gate.shape[1],)
-        if call.args.get("keep"):
-            size = x.size // x.shape[-1] * gate.shape[1]
-            call.args["gate"], call.args["up"] = (call.device.allocate(x.dtype, size) for _ in range(2))
-        return call.withInputs([_new_output(call.device, x.dtype, shape, overwritten=True), x, gate, up])
+        if gate.ndc.asDense() is None or up.ndc.asDense() is None:
+            if gate.ndc.asDenseColumns() is None or up.ndc.asDenseColumns() is None:
+                gate, up = as_dense(gate), as_dense(up)
+        N = gate.ndc.shape[1]
+        if call.args["keep"]:
+            size = x.ndc.size // K * N
+            call.args["gate"], call.args["up"] = call.device.allocate(x.dtype, size), call.device.allocate(x.dtype, size)
+        call.inputs = [_new_output(call.device, x.dtype, x.ndc.shape[:-1] + (N,), overwritten=True), x, gate, up]
+        return call
 
 
 class Operation:

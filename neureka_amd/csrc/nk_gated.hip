@@ -50,9 +50,9 @@ struct Product {
     int tiles_m, tiles_n, steps_per_part;   // a part: that many steps of BK along the contraction
     int64_t part_stride;                // elements from one part's results to the next's
     int fun;
-    T* out[3];                          // GATED: H, gate, up; STORE: the product (both halves)
+    T* out[3];                          // GATED: H, gate, up; STORE: the product (both halves); SUM: their sum
 };
-enum { STORE = 0, GATED = 1 };
+enum { STORE = 0, GATED = 1, SUM = 2 };      // SUM: both halves added into one result
 
 template <typename T> struct Quad;
 template <> struct Quad<float> {        // register v of lane l: row 4 (l / 16) + v, column l % 16 of a 16 x 16 tile
@@ -477,6 +477,152 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
     }
 }
 
+// ---- few rows ----------------------------------------------------------------------------------------------------------
+// Up to 64 rows the weights' bytes bound the products, so they go from memory straight into the registers of the matrix
+// instructions (16 x 16 x 4, of the element type itself), each element once.  A wavefront owns 16 CW columns of both products and
+// RT x 16 rows; the block's WAVES wavefronts share the contraction in chunks of KC, chunk after chunk in turn, and add their sums
+// through LDS in order.  Inside a chunk quarter q of a wavefront takes l from V q on, so that a lane's V values of A (and of
+// weights stored along l) are one 16-byte load.
+template <typename T, int RT, int CW, int WAVES, bool ALONG, int EPI>
+__global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const Product<T> g) {
+    typedef Quad<T> Q;
+    typedef typename Q::Acc Acc;
+    constexpr int V = 16 / sizeof(T), KC = 4 * V, U = RT > 2 ? 1 : 2, NA = EPI == GATED ? 1 : 2;      // U chunks are loaded at a time
+    typedef T VecV __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, c = lane & 15, q = lane >> 4;
+    const unsigned groups = (unsigned)g.tiles_n, part = blockIdx.x / groups;
+    int none, group;
+    own_tile(blockIdx.x - part * groups, groups, 1, g.tiles_n, none, group);
+    const int n0 = group * 16 * CW;
+    const T *brow[2][CW], *arow[NA][RT];                    // ALONG: the lane's CW columns; else brow[.][0]: column n0 + c CW
+#pragma unroll
+    for (int p = 0; p < 2; p++)
+#pragma unroll
+        for (int j = 0; j < CW; j++) {
+            const int n = ALONG ? n0 + j * 16 + c : n0 + c * CW + j;
+            brow[p][j] = g.B[p] + (int64_t)(n < g.cols ? n : g.cols - 1) * (ALONG ? g.ldb : 1);
+        }
+#pragma unroll
+    for (int p = 0; p < NA; p++)
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            const int m = r * 16 + c;
+            arow[p][r] = g.A[p] + (int64_t)(m < g.rows ? m : g.rows - 1) * g.lda;
+        }
+    Acc acc[2][RT][CW] = {};
+    struct Chunk { T a[NA][RT][V], b[2][CW][V]; };
+    const auto load = [&](Chunk& k, int64_t l0) {            // a chunk that exists whole: no branch, so that the requests of several overlap
+        const int64_t l = l0 + q * V;
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            if constexpr (ALONG) {
+#pragma unroll
+                for (int j = 0; j < CW; j++) {
+                    const VecV w = *(const VecV*)(brow[p][j] + l);
+#pragma unroll
+                    for (int s = 0; s < V; s++) k.b[p][j][s] = w[s];
+                }
+            } else
+#pragma unroll
+                for (int s = 0; s < V; s++)
+#pragma unroll
+                    for (int j = 0; j < CW; j++) k.b[p][j][s] = brow[p][j][(l + s) * g.ldb];
+        }
+#pragma unroll
+        for (int p = 0; p < NA; p++)
+#pragma unroll
+            for (int r = 0; r < RT; r++) {
+                const VecV x = *(const VecV*)(arow[p][r] + l);
+#pragma unroll
+                for (int s = 0; s < V; s++) k.a[p][r][s] = x[s];
+            }
+    };
+    const auto load_rest = [&](Chunk& k, int64_t l0) {       // the last one, zeros past the end
+        const int64_t l = l0 + q * V;
+#pragma unroll
+        for (int s = 0; s < V; s++) {
+            const bool in = l + s < g.inner;
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int j = 0; j < CW; j++) k.b[p][j][s] = in ? brow[p][j][(l + s) * (ALONG ? 1 : g.ldb)] : T(0);
+#pragma unroll
+            for (int p = 0; p < NA; p++)
+#pragma unroll
+                for (int r = 0; r < RT; r++) k.a[p][r][s] = in ? arow[p][r][l + s] : T(0);
+        }
+    };
+    const auto multiply = [&](const Chunk& k) {
+#pragma unroll
+        for (int s = 0; s < V; s++)
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int p = 0; p < 2; p++)
+#pragma unroll
+                    for (int j = 0; j < CW; j++) acc[p][r][j] = Q::mma(k.a[NA == 1 ? 0 : p][r][s], k.b[p][j][s], acc[p][r][j]);
+    };
+    // whole chunks first + wave, first + wave + WAVES, ... below last; what is left over belongs to the last part's first wavefront
+    const int whole = g.inner / KC, first = (int)part * g.steps_per_part < whole ? (int)part * g.steps_per_part : whole;
+    const int last = first + g.steps_per_part < whole ? first + g.steps_per_part : whole;
+    const int mine = last - first - wave > 0 ? (last - first - wave + WAVES - 1) / WAVES : 0;
+    const auto at = [&](int i) { return (int64_t)(first + wave + i * WAVES) * KC; };
+    int i = 0;
+    if (mine >= U) {
+        Chunk now[U], next[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) load(now[u], at(u));
+        for (; i + 2 * U <= mine; i += U) {
+#pragma unroll
+            for (int u = 0; u < U; u++) load(next[u], at(i + U + u));
+            __builtin_amdgcn_sched_barrier(0);               // the requests go out before the products of the chunks that are here
+#pragma unroll
+            for (int u = 0; u < U; u++) multiply(now[u]);
+#pragma unroll
+            for (int u = 0; u < U; u++) now[u] = next[u];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) multiply(now[u]);
+        i += U;
+    }
+    Chunk one;
+    for (; i < mine; i++) { load(one, at(i)); multiply(one); }
+    if (wave == 0 && last == whole && g.inner % KC != 0) { load_rest(one, (int64_t)whole * KC); multiply(one); }
+
+    // the wavefronts' sums: [wave][product][row tile][column fragment][lane], a fragment's four values at a time
+    Acc* const sums = (Acc*)lds;
+    constexpr int FRAGMENTS = RT * CW;
+#pragma unroll
+    for (int p = 0; p < 2; p++)
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int j = 0; j < CW; j++) sums[((wave * 2 + p) * FRAGMENTS + r * CW + j) * 64 + lane] = acc[p][r][j];
+    __syncthreads();
+    for (int f = wave; f < FRAGMENTS; f += WAVES) {
+        Acc x = sums[f * 64 + lane], y = sums[(FRAGMENTS + f) * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) {
+            x += sums[((w * 2) * FRAGMENTS + f) * 64 + lane];
+            y += sums[((w * 2 + 1) * FRAGMENTS + f) * 64 + lane];
+        }
+        const int r = f / CW, j = f % CW, n = ALONG ? n0 + j * 16 + c : n0 + c * CW + j;
+        if (n >= g.cols) continue;
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const int m = r * 16 + Q::row(lane, v);
+            if (m >= g.rows) continue;
+            const int64_t o = (int64_t)m * g.cols + n + (int64_t)part * g.part_stride;
+            if constexpr (EPI == GATED) {
+                g.out[0][o] = gated_fun(g.fun, x[v]) * y[v];
+                if (g.out[1]) { g.out[1][o] = x[v]; g.out[2][o] = y[v]; }
+            } else if constexpr (EPI == SUM) g.out[0][o] = x[v] + y[v];
+            else { g.out[0][o] = x[v]; g.out[1][o] = y[v]; }
+        }
+    }
+}
+
 // ---- parts of the contraction, added in order -----------------------------------------------------------------------
 // partial: [parts][halves][n]; halves 2: the pair of products
 template <typename T, bool PAIRED, int EPI>
@@ -492,7 +638,8 @@ __global__ __launch_bounds__(256) void product_join_kernel(const T* __restrict__
     if constexpr (EPI == GATED) {
         out0[i] = gated_fun(fun, x) * y;
         if (out1) { out1[i] = x; out2[i] = y; }
-    } else {
+    } else if constexpr (EPI == SUM) out0[i] = x + y;
+    else {
         out0[i] = x;
         if (PAIRED) out1[i] = y;
     }
@@ -569,14 +716,74 @@ static void launch_product(Device* dev, Product<T> g, const Split& s, bool a_alo
     hipLaunchKernelGGL((product_join_kernel<T, PAIRED, EPI>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, dev->stream, partial, s.parts, n, g.fun, out[0], out[1], out[2]);
 }
 
+// The products of up to 64 rows.  one_a: both products have the same A (GATED), else each has its own (SUM).
+struct FewPlan { int row_tiles, groups, parts, steps_per_part; };
+template <typename T>
+static FewPlan few_plan(const Device* dev, int64_t rows, int64_t cols, int64_t inner) {
+    FewPlan f;
+    const int64_t cus = dev->props.multiProcessorCount, chunk = 64 / (int64_t)sizeof(T), chunks = inner / chunk;
+    f.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    f.groups = (int)((cols + 15) / 16);
+    // parts of the contraction for columns that fill less than half of the units, 32 chunks per part at least
+    int64_t parts = f.groups * 2 > cus ? 1 : cus / f.groups;
+    if (parts > chunks / 32) parts = chunks / 32 > 0 ? chunks / 32 : 1;
+    f.steps_per_part = chunks ? (int)((chunks + parts - 1) / parts) : 1;
+    f.parts = chunks ? (int)((chunks + f.steps_per_part - 1) / f.steps_per_part) : 1;
+    return f;
+}
+static uint64_t few_partial_elements(const FewPlan& f, int64_t rows, int64_t cols) { return f.parts > 1 ? (uint64_t)f.parts * 2 * rows * cols : 0; }
+
+template <typename T, int EPI>
+static int launch_few(Device* dev, Product<T> g, const FewPlan& f, bool along, T* partial) {
+    constexpr int WAVES = 8;
+    g.tiles_n = f.groups; g.steps_per_part = f.steps_per_part;
+    const int64_t n = (int64_t)g.rows * g.cols;
+    T* const out[3] = {g.out[0], g.out[1], g.out[2]};
+    if (f.parts > 1) { g.out[0] = partial; g.out[1] = partial + n; g.out[2] = nullptr; g.part_stride = 2 * n; }
+    hipError_t refused = hipSuccess;
+    const auto go = [&](auto rt, auto epi) {
+        constexpr int RT = decltype(rt)::value, E = decltype(epi)::value;
+        const unsigned bytes = WAVES * 2 * RT * 64 * 4 * sizeof(T);
+        const auto run = [&](auto kernel) {
+            if (bytes > 65536) refused = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+            if (refused == hipSuccess) hipLaunchKernelGGL(kernel, dim3((unsigned)(f.groups * f.parts)), dim3(WAVES * 64), bytes, dev->stream, g);
+        };
+        if (along) run(few_rows_kernel<T, RT, 1, WAVES, true, E>);
+        else       run(few_rows_kernel<T, RT, 1, WAVES, false, E>);
+    };
+    const auto rows = [&](auto epi) {
+        if (f.row_tiles == 1)      go(std::integral_constant<int, 1>(), epi);
+        else if (f.row_tiles == 2) go(std::integral_constant<int, 2>(), epi);
+        else                       go(std::integral_constant<int, 4>(), epi);
+    };
+    if (f.parts == 1) rows(std::integral_constant<int, EPI>());
+    else {
+        // (with parts the two products of a GATED call still share their A, which STORE does not know: A[1] = A[0])
+        g.A[1] = g.A[1] ? g.A[1] : g.A[0];
+        rows(std::integral_constant<int, STORE>());
+        hipLaunchKernelGGL((product_join_kernel<T, true, EPI>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, dev->stream, partial, f.parts, n, g.fun, out[0], out[1], out[2]);
+    }
+    NK_HIP(refused);
+    return NK_OK;
+}
+
 template <typename T>
 static int gated_forward(Device* dev, int fun, bool along, int64_t M, int64_t K, int64_t N, const T* X, const T* Wg, const T* Wu, T* H, T* gate, T* up) {
     Product<T> g{};
     g.A[0] = X; g.lda = K; g.B[0] = Wg; g.B[1] = Wu; g.ldb = along ? K : N;
     g.rows = (int)M; g.cols = (int)N; g.inner = (int)K; g.segments = 1; g.fun = fun;
     g.out[0] = H; g.out[1] = gate; g.out[2] = up;
-    const Split s = plan<T>(dev, true, M, N, K, 1);
     void* ws = nullptr;
+    if (M <= 64) {
+        const FewPlan f = few_plan<T>(dev, M, N, K);
+        if (const uint64_t need = few_partial_elements(f, M, N))
+            if (int e = workspace(dev, need * sizeof(T), &ws)) return e;
+        if (int e = launch_few<T, GATED>(dev, g, f, along, (T*)ws)) return e;
+        NK_HIP(hipGetLastError());
+        set_path(f.parts > 1 ? "gated_few_rows_split" : "gated_few_rows");
+        return NK_OK;
+    }
+    const Split s = plan<T>(dev, true, M, N, K, 1);
     if (const uint64_t need = partial_elements(s, true, M, N))
         if (int e = workspace(dev, need * sizeof(T), &ws)) return e;
     launch_product<T, true, GATED>(dev, g, s, true, along, (T*)ws);
@@ -590,7 +797,8 @@ static int gated_backward(Device* dev, int fun, bool along, int64_t M, int64_t K
                           const T* E, T* dX, T* dWg, T* dWu) {
     const int64_t n = M * N;
     const Split sx = plan<T>(dev, false, M, K, N, 2), sw = plan<T>(dev, true, K, N, M, 1);
-    const uint64_t px = dX ? partial_elements(sx, false, M, K) : 0, pw = dWg ? partial_elements(sw, true, K, N) : 0;
+    const FewPlan few = few_plan<T>(dev, M, K, N);
+    const uint64_t px = dX ? M <= 64 ? few_partial_elements(few, M, K) : partial_elements(sx, false, M, K) : 0, pw = dWg ? partial_elements(sw, true, K, N) : 0;
     void* ws = nullptr;
     if (int e = workspace(dev, (2 * (uint64_t)n + (px > pw ? px : pw)) * sizeof(T), &ws)) return e;
     T *const dg = (T*)ws, *const du = dg + n, *const partial = du + n;
@@ -600,7 +808,8 @@ static int gated_backward(Device* dev, int fun, bool along, int64_t M, int64_t K
         g.A[0] = dg; g.A[1] = du; g.lda = N; g.B[0] = Wg; g.B[1] = Wu; g.ldb = along ? K : N;
         g.rows = (int)M; g.cols = (int)K; g.inner = (int)N; g.segments = 2;
         g.out[0] = dX;
-        launch_product<T, false, STORE>(dev, g, sx, true, !along, partial);      // (weights stored by row have neighbours along N)
+        if (M <= 64) { if (int e = launch_few<T, SUM>(dev, g, few, !along, partial)) return e; }
+        else launch_product<T, false, STORE>(dev, g, sx, true, !along, partial);      // (weights stored by row have neighbours along N)
     }
     if (dWg) {
         Product<T> g{};

@@ -21,6 +21,7 @@ _INT_CODES = {np.dtype(np.int32): 2, np.dtype(np.int64): 3, np.dtype(np.int16): 
 
 
 _ITEM_SIZES = {np.float32: 4, np.float64: 8, np.int32: 4, np.int64: 8, np.int16: 2, np.int8: 1, np.uint8: 1}
+_ITEM_SIZES.update({np.dtype(k): v for k, v in list(_ITEM_SIZES.items())})
 _FLOAT_CODES = {np.float32: _lib.F32, np.float64: _lib.F64, np.dtype(np.float32): _lib.F32, np.dtype(np.float64): _lib.F64}
 
 

@@ -40,19 +40,16 @@ def execute(op_id: str, inputs: Sequence[Tensor], d: int = -1, record: bool = Tr
     ctx = backend()
     operation = ctx.getOperation(op_id)
     device = _device_for(inputs)
+    if op_id in SUBLAYER_OPERATIONS:
+        return _execute_sublayer(operation, device, inputs, d, record, args or {})
     if op_id == "left_inline":               # operations/other/AssignLeft.java:103-114: inline, no autograd
         if d >= 0:
             raise IllegalArgumentException("Assignment does not support autograd!")
         record = False
     parents = list(inputs)                   # the tensors the caller holds: gradients attach to these
-    if op_id in SUBLAYER_OPERATIONS and d >= 0:
-        raise IllegalArgumentException(f"'{op_id}' has no elementwise derivative; its gradients come from backward()")
-    if len(inputs) > 1 and op_id != "dot" and op_id not in SUBLAYER_OPERATIONS and any(len(t.ndc.shape) != len(inputs[0].ndc.shape) for t in inputs):
+    if len(inputs) > 1 and op_id != "dot" and any(len(t.ndc.shape) != len(inputs[0].ndc.shape) for t in inputs):
         inputs = make_fit(list(inputs))      # FunctionNode.execute pads ranks first (FunctionNode.java:92-93)
-    recorded = record and d < 0 and any(t.rqsGradient() or t._node is not None for t in parents)
     call = ExecutionCall(device, operation, list(inputs), d)
-    if args is not None or op_id in SUBLAYER_OPERATIONS:
-        call.args = dict(args or {}, keep=recorded)
     call.algorithm = operation.getAlgorithmFor(call)
 
     def run(c: ExecutionCall):
@@ -63,9 +60,21 @@ def execute(op_id: str, inputs: Sequence[Tensor], d: int = -1, record: bool = Tr
         return execute_device_algorithm(c), c
 
     result, prepared = execute_on_common_device(call, run)
+    if record and d < 0 and any(t.rqsGradient() or t._node is not None for t in parents):
+        result._node = _graph_node(op_id, prepared, parents, result)
+    return result
+
+
+def _execute_sublayer(operation, device, parents: Sequence[Tensor], d: int, record: bool, args: dict) -> Tensor:
+    """execute() for SUBLAYER_OPERATIONS: one algorithm each, which prepares ranks and views itself."""
+    if d >= 0:
+        raise IllegalArgumentException(f"'{operation.identifier}' has no elementwise derivative; its gradients come from backward()")
+    wanted = [t._rqs_gradient or t._node is not None for t in parents]
+    recorded = record and True in wanted
+    call = ExecutionCall(device, operation, list(parents), -1, operation.algorithms[0], dict(args, keep=recorded))
+    result = execute_on_common_device(call, lambda c: execute_device_algorithm(c.algorithm.prepare(c)))
     if recorded:
-        joint = _joint_gradients(op_id, prepared, parents) if op_id in SUBLAYER_OPERATIONS else None
-        result._node = GraphNode(parents, (), joint) if joint else _graph_node(op_id, prepared, parents, result)
+        result._node = GraphNode(parents, (), _joint_gradients(call, parents, wanted))
     return result
 
 
@@ -81,33 +90,34 @@ def _graph_node(op_id: str, call: ExecutionCall, inputs: List[Tensor], result: T
     return GraphNode(inputs, actions)
 
 
-def _joint_gradients(op_id: str, call: ExecutionCall, parents: List[Tensor]):
+def _joint_gradients(call: ExecutionCall, parents: Sequence[Tensor], wanted: List[bool]):
     """For operations whose gradients share their work: error of the result -> one gradient (or None) per parent."""
-    device, args = call.device, call.args
-    drn, *operands = call.inputs                  # as the kernel saw them
-    shape, dtype = drn.shape, drn.dtype
-    wanted = [t.rqsGradient() or t._node is not None for t in parents]
+    # (the node belongs to the result: nothing here may hold the result, or the call whose drain it is -- a cycle would keep every
+    # buffer until the garbage collector comes by)
+    device, operation, args = call.device, call.operation, call.args
+    op_id, operands = operation.identifier, call.inputs[1:]      # as the kernel saw them
+    shape, dtype, parent_shapes = call.inputs[0].shape, call.inputs[0].dtype, [t.shape for t in parents]
 
     def act(error: Tensor) -> List[Optional[Tensor]]:
         if error.shape != shape or error.dtype != dtype:
             raise IllegalArgumentException(f"the error of a {dtype}{list(shape)} result cannot be {error.dtype}{list(error.shape)}")
         # operands that live on the host are stored for the launch and restored afterwards
-        run = ExecutionCall(device, call.operation, operands + [error], args=args)
+        run = ExecutionCall(device, operation, operands + [error])
         return execute_on_common_device(run, lambda c: gradients(error))
 
     def gradients(error: Tensor) -> List[Optional[Tensor]]:
-        if op_id == "dropout":
-            return [execute("dropout", [error], record=False, args={k: args[k] for k in ("probability", "seed", "offset")})]
-        error = as_dense(error)
-        out = [Tensor._on_device(device, dtype, p.shape, zeroed=False) if w else None for p, w in zip(parents, wanted)]
-        if op_id == "layerNorm":
-            src, gain, _ = operands
-            device.launch_layer_norm_backward(src, gain, args["mean"], args["rstd"], error, *out)
-            return out
-        d_x, d_gate, d_up = out
-        if (d_gate is None) != (d_up is None):    # the kernel computes both
-            d_gate, d_up = (Tensor._on_device(device, dtype, parents[1].shape, zeroed=False) if t is None else t for t in (d_gate, d_up))
-        device.launch_gated_matmul_backward(args["activation"], *operands, args["gate"], args["up"], error, d_x, d_gate, d_up)
+        if error._virtual:
+            error.setIsVirtual(False)
+        out = [Tensor._on_device(device, dtype, s, zeroed=False) if w else None for s, w in zip(parent_shapes, wanted)]
+        if op_id == "dropout":                    # the same mask on the error
+            device.launch_dropout(out[0], error, args["probability"], args["seed"], args["offset"])
+        elif op_id == "layerNorm":
+            device.launch_layer_norm_backward(operands[0], operands[1], args["mean"], args["rstd"], as_dense(error), *out)
+        else:
+            d_x, d_gate, d_up = out
+            if (d_gate is None) != (d_up is None):               # the kernel computes both
+                d_gate, d_up = (Tensor._on_device(device, dtype, parent_shapes[1], zeroed=False) if t is None else t for t in (d_gate, d_up))
+            device.launch_gated_matmul_backward(args["activation"], *operands, args["gate"], args["up"], as_dense(error), d_x, d_gate, d_up)
         return out
     return act
 

@@ -113,7 +113,7 @@ class NDConfiguration:
     def rank(self) -> int:
         return len(self.shape)
 
-    @property
+    @functools.cached_property
     def size(self) -> int:
         s = 1
         for d in self.shape:
@@ -204,11 +204,12 @@ class NDConfiguration:
     def asRows(self):
         """(first element, rows, columns, elements from one row to the next) where the elements of the last axis lie next
         to each other and the rows -- the leading axes in row-major order -- lie one pitch apart; None for any other view."""
-        if "_rows" not in self.__dict__:
-            object.__setattr__(self, "_rows", None if self.virtual else self._findRows())
-        return self.__dict__["_rows"]
+        return self._rows
 
-    def _findRows(self):
+    @functools.cached_property
+    def _rows(self):
+        if self.virtual:
+            return None
         steps = [s * p for s, p in zip(self.strides, self.spread)]
         base = sum(o * s for o, s in zip(self.offset, self.strides))
         cols = self.shape[-1]
@@ -228,7 +229,11 @@ class NDConfiguration:
 
     def asDense(self):
         """First element of a view whose elements lie next to each other in row-major order; None for any other view."""
-        rows = self.asRows()
+        return self._dense
+
+    @functools.cached_property
+    def _dense(self):
+        rows = self._rows
         return rows[0] if rows is not None and (rows[1] == 1 or rows[3] == rows[2]) else None
 
     def asDenseColumns(self):

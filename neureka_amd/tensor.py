@@ -381,11 +381,11 @@ class GraphNode:
 
 
 def _backward(result: Tensor, error: Tensor) -> None:
-    from .function import execute
     if result._rqs_gradient:
         if result.gradient is None:
             result.gradient = error
         else:
+            from .function import execute
             result.gradient = execute("add", [result.gradient, error], record=False)
     node = result._node
     if node is None:
