@@ -50,6 +50,7 @@ struct Product {
     int tiles_m, tiles_n, steps_per_part;   // a part: that many steps of BK along the contraction
     int64_t part_stride;                // elements from one part's results to the next's
     int fun;
+    const int *a_scale, *b_scale[2];    // binary exponents of the rows of A and of B (per half), or null: see split_product_kernel
     T* out[3];                          // GATED: H, gate, up; STORE: the product (both halves); SUM: their sum
 };
 enum { STORE = 0, GATED = 1, SUM = 2 };      // SUM: both halves added into one result
@@ -180,17 +181,29 @@ __global__ __launch_bounds__(256) void product_kernel(const Product<T> g) {
         }
 }
 
-// ---- f32 products on the bf16 matrix cores ------------------------------------------------------------------------
-// A float is the sum of three bfloat16 numbers, each the rest of the ones before rounded to nearest: 3 x 8 bits hold its 24 (below
-// 2^-110 the last of them leaves bfloat16's range, and the sum is off by at most 2^-134).  Of the nine partial products the
-// six largest are added, x0 y0, x0 y1, x1 y0, x1 y1, x0 y2, x2 y0; the other three are at most 2^-26 of x y each, less than the
-// rounding of an f32 product.  Partial products are exact and their sums are f32, as in a product of floats.  The bf16
-// instruction does 16 times the work of the f32 one per cycle, so six of them cost 6 / 16 of one f32 product.
+// ---- f32 products on the 16-bit matrix cores --------------------------------------------------------------------------
+// The 16-bit instructions do 16 times the work of the f32 one per cycle and add exact partial products in f32, so a product of
+// sums of 16-bit numbers costs less than the product of the floats they make up, at the same accuracy.  Two ways (PLANES):
 //
-// A non-finite operand has no such sum (infinity - infinity), so a wavefront that finds a non-finite result computes its tile
-// once more with the f32 instruction, straight from memory: what comes out is what f32 arithmetic gives.
+// 3: bfloat16, any operands.  A float is the sum of three, each the rest of the ones before rounded to nearest: 3 x 8 bits hold its 24
+// (below 2^-110 the last leaves bfloat16's range: off by at most 2^-134).  The six largest of the nine partial products are added,
+// x0 y0, x0 y1, x1 y0, x1 y1, x0 y2, x2 y0; the rest is at most 2^-26 of x y each.  A non-finite operand has no such sum
+// (infinity - infinity), so a wavefront that finds a non-finite result computes its tile once more with the f32
+// instruction, straight from memory: what comes out is what f32 arithmetic gives.
+//
+// 2: half precision, half as many partial products: x0 y0, x0 y1, x1 y0.  Two halves hold a float to 2^-23 of it (2^-25 on average)
+// and x1 y1 is at most 2^-22 of x y (2^-25 on average, of either sign), as long as they stay within the type's few binades.
+// So a launch before finds, for every row of A and of B, the power of two that brings its largest magnitude below
+// 2^15; what is 2^-16 of that or more keeps all its bits, and smaller numbers are off by at most 2^-40 of the largest.
+// A row where that could show -- more than a quarter of its 64 stretches hold nothing beyond 2^-16 of the largest (and are not all
+// zero), or an infinity or NaN -- is marked, and tiles with a marked row are left to a launch with three planes.
+constexpr int64_t TWO_PLANES_FROM = (int64_t)1 << 32;        // multiply-adds
+constexpr int MARKED = 1 << 30;                              // in place of a row's exponent
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
@@ -208,28 +221,143 @@ __device__ __forceinline__ void split_pair(float x, float y, unsigned (&p)[3]) {
         }
     }
 }
+// two scaled floats -> their two pairs of halves
+__device__ __forceinline__ void split_pair(float x, float y, unsigned (&p)[2]) {
+    const f16x2 high = {(_Float16)x, (_Float16)y};
+    const f16x2 low = {(_Float16)(x - (float)high[0]), (_Float16)(y - (float)high[1])};
+    p[0] = __builtin_bit_cast(unsigned, high);
+    p[1] = __builtin_bit_cast(unsigned, low);
+}
+template <int PLANES> struct Partial;
+template <> struct Partial<3> {
+    static constexpr int N = 6, A[N] = {0, 1, 2, 0, 1, 0}, B[N] = {0, 0, 0, 1, 1, 2};
+    static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Partial<2> {
+    static constexpr int N = 3, A[N] = {0, 1, 0}, B[N] = {0, 0, 1};
+    static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
 
-// LDS holds an operand's slice (WIDTH rows x 16 l) as three planes of fragments of 32 rows x 16 l in the order in which the
-// lanes of v_mfma_f32_32x32x16_bf16 take them: lane l gets the 8 values of row l % 32 from 8 (l / 32) on, 16 bytes.  The upper half's
+// The exponents of up to three operands' rows (`count` rows of `length`, together with those of a second matrix where there is
+// one), blocks dealt out operand by operand.  Rows that lie along memory: a wavefront each, 64 stretches of every 64th 4
+// elements.  Rows across memory: 32 of them per block, 64 stretches of every 64th element.  Read once at memory speed.
+struct ScaleJob { const float* p[2]; int64_t ld; int count, length; bool along; int* out; unsigned blocks; };
+struct ScaleJobs { ScaleJob job[3]; int n; };
+__device__ __forceinline__ unsigned magnitude(float x) { return __builtin_bit_cast(unsigned, x) & 0x7fffffffu; }
+__device__ __forceinline__ int exponent_for(unsigned largest, int low, int some) {      // low of some non-zero stretches are far below the largest
+    if (largest >= 0x7f800000u || 4 * low > some) return MARKED;
+    const int e = 14 + 127 - (int)(largest >> 23);
+    return largest == 0 ? 0 : e < 126 ? e : 126;
+}
+__device__ __forceinline__ bool far_below(unsigned m, unsigned largest) { return m != 0 && (m >> 23) + 16 < (largest >> 23); }
+
+__global__ __launch_bounds__(512) void operand_scales_kernel(const ScaleJobs jobs) {
+    unsigned block = blockIdx.x;
+    int which = 0;
+    while (which + 1 < jobs.n && block >= jobs.job[which].blocks) block -= jobs.job[which++].blocks;
+    const ScaleJob j = jobs.job[which];
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    if (j.along) {
+        const int row = (int)block * 8 + wave;
+        if (row >= j.count) return;
+        unsigned m = 0;
+        for (int k = 0; k < 2; k++) {
+            if (!j.p[k]) continue;
+            const float* const at = j.p[k] + (int64_t)row * j.ld;
+            int i = lane * 4;
+#pragma unroll 4
+            for (; i + 4 <= j.length; i += 256) {
+                const f32x4 v = *(const f32x4_any*)(at + i);
+#pragma unroll
+                for (int e = 0; e < 4; e++) { const unsigned u = magnitude(v[e]); m = u > m ? u : m; }
+            }
+            for (; i < j.length; i++) { const unsigned u = magnitude(at[i]); m = u > m ? u : m; }
+        }
+        unsigned largest = m;
+#pragma unroll
+        for (int step = 32; step > 0; step >>= 1) { const unsigned o = __shfl_xor(largest, step); largest = o > largest ? o : largest; }
+        const int low = __popcll(__ballot(far_below(m, largest))), some = __popcll(__ballot(m != 0));
+        if (lane == 0) j.out[row] = exponent_for(largest, low, some);
+        return;
+    }
+    // lane: 4 neighbouring rows c .. c + 3 of the block's 32, stretch 8 wave + lane / 8
+    __shared__ unsigned waves_largest[8][32];
+    __shared__ unsigned waves_low[8][8], waves_some[8][8];          // counts of 4 rows, a byte each
+    const int q = lane & 7, c = (int)block * 32 + q * 4, first = wave * 8 + (lane >> 3);
+    unsigned m[4] = {0, 0, 0, 0};
+    for (int k = 0; k < 2; k++) {
+        if (!j.p[k]) continue;
+        if (c + 4 <= j.count) {
+            const float* const at = j.p[k] + c;
+#pragma unroll 4
+            for (int l = first; l < j.length; l += 64) {
+                const f32x4 v = *(const f32x4_any*)(at + (int64_t)l * j.ld);
+#pragma unroll
+                for (int e = 0; e < 4; e++) { const unsigned u = magnitude(v[e]); m[e] = u > m[e] ? u : m[e]; }
+            }
+        } else
+            for (int l = first; l < j.length; l += 64)
+#pragma unroll
+                for (int e = 0; e < 4; e++) if (c + e < j.count) { const unsigned u = magnitude(j.p[k][(int64_t)l * j.ld + c + e]); m[e] = u > m[e] ? u : m[e]; }
+    }
+    unsigned largest[4] = {m[0], m[1], m[2], m[3]};
+#pragma unroll
+    for (int step = 8; step < 64; step <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; e++) { const unsigned o = __shfl_xor(largest[e], step); largest[e] = o > largest[e] ? o : largest[e]; }
+    if (lane < 8)
+#pragma unroll
+        for (int e = 0; e < 4; e++) waves_largest[wave][q * 4 + e] = largest[e];
+    __syncthreads();
+    unsigned low = 0, some = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        for (int w = 0; w < 8; w++) { const unsigned o = waves_largest[w][q * 4 + e]; largest[e] = o > largest[e] ? o : largest[e]; }
+        low |= (unsigned)far_below(m[e], largest[e]) << (8 * e);
+        some |= (unsigned)(m[e] != 0) << (8 * e);
+    }
+#pragma unroll
+    for (int step = 8; step < 64; step <<= 1) { low += __shfl_xor(low, step); some += __shfl_xor(some, step); }
+    if (lane < 8) { waves_low[wave][q] = low; waves_some[wave][q] = some; }
+    __syncthreads();
+    if (wave == 0 && lane < 8) {
+        low = some = 0;
+        for (int w = 0; w < 8; w++) { low += waves_low[w][q]; some += waves_some[w][q]; }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (c + e < j.count) j.out[c + e] = exponent_for(largest[e], (low >> (8 * e)) & 255, (some >> (8 * e)) & 255);
+    }
+}
+
+// LDS holds an operand's slice (WIDTH rows x 16 l) as PLANES planes of fragments of 32 rows x 16 l in the order in which the
+// lanes of v_mfma_f32_32x32x16 take them: lane l gets the 8 values of row l % 32 from 8 (l / 32) on, 16 bytes.  The upper half's
 // rows are rotated by 8 (row ^ 8) so that the writes below do not meet in one bank; a read is 1 KiB without a gap either way.
-template <int WIDTH, bool ALONG, int THREADS>
+template <int PLANES, int WIDTH, bool ALONG, int THREADS>
 struct SplitShare {
     static constexpr int E = WIDTH * 16 / THREADS;          // elements per thread: 4 or 8
     static constexpr unsigned PLANE = WIDTH * 32;           // bytes
     static_assert(E == 4 || E == 8, "a thread moves one or two times four elements");
     float v[E];
     const float* base[E / 4];                               // ALONG: the thread's rows; else: its column (base[0])
+    float scale[E / 4];                                     // two planes: their powers of two
     int l_of;                                               // first l of the thread inside a slice
 
-    __device__ __forceinline__ void place(const float* a, int64_t ld, int first, int count, int t, int half_of_columns, const float* other) {
+    __device__ __forceinline__ void place(const float* a, int64_t ld, int first, int count, int t, int half_of_columns, const float* other,
+                                          const int* exponents, const int* other_exponents) {
         // half_of_columns > 0: rows from there on belong to the second matrix of a pair
 #pragma unroll
         for (int u = 0; u < E / 4; u++) {
             int r = ALONG ? (t + u * THREADS) >> 2 : t % WIDTH;
             const float* from = a;
-            if (half_of_columns > 0 && r >= half_of_columns) { r -= half_of_columns; from = other; }
+            const int* exponent = exponents;
+            if (half_of_columns > 0 && r >= half_of_columns) { r -= half_of_columns; from = other; exponent = other_exponents; }
             const int64_t row = first + r < count ? first + r : count - 1;       // past the end: the last one, its results are not stored
             base[u] = from + row * (ALONG ? ld : 1);
+            if constexpr (PLANES == 2) scale[u] = __builtin_bit_cast(float, (unsigned)(exponent[row] + 127) << 23);
         }
         l_of = ALONG ? (t & 3) * 4 : __builtin_amdgcn_readfirstlane(t / WIDTH) * E;
     }
@@ -257,9 +385,12 @@ struct SplitShare {
         }
     }
     __device__ __forceinline__ void store(unsigned char* lds, int t) const {
-        unsigned p[E / 2][3];
+        unsigned p[E / 2][PLANES];
 #pragma unroll
-        for (int e = 0; e < E / 2; e++) split_pair(v[2 * e], v[2 * e + 1], p[e]);
+        for (int e = 0; e < E / 2; e++) {
+            const float by = PLANES == 2 ? scale[ALONG ? e / 2 : 0] : 1.0f;
+            split_pair(PLANES == 2 ? v[2 * e] * by : v[2 * e], PLANES == 2 ? v[2 * e + 1] * by : v[2 * e + 1], p[e]);
+        }
         if constexpr (ALONG) {
             const int q = t & 3, high = q >> 1;
 #pragma unroll
@@ -267,13 +398,13 @@ struct SplitShare {
                 const int r = (t + u * THREADS) >> 2;
                 unsigned char* const at = lds + (r >> 5) * 1024 + high * 512 + ((r & 31) ^ (high * 8)) * 16 + (q & 1) * 8;
 #pragma unroll
-                for (int k = 0; k < 3; k++) *(uint2*)(at + k * PLANE) = make_uint2(p[u * 2][k], p[u * 2 + 1][k]);
+                for (int k = 0; k < PLANES; k++) *(uint2*)(at + k * PLANE) = make_uint2(p[u * 2][k], p[u * 2 + 1][k]);
             }
         } else {
             const int r = t % WIDTH, l = l_of, high = l >> 3;
             unsigned char* const at = lds + (r >> 5) * 1024 + high * 512 + ((r & 31) ^ (high * 8)) * 16 + (l & 4) * 2;
 #pragma unroll
-            for (int k = 0; k < 3; k++) {
+            for (int k = 0; k < PLANES; k++) {
                 if constexpr (E == 8) *(uint4*)(at + k * PLANE) = make_uint4(p[0][k], p[1][k], p[2][k], p[3][k]);
                 else                  *(uint2*)(at + k * PLANE) = make_uint2(p[0][k], p[1][k]);
             }
@@ -288,23 +419,37 @@ __device__ __forceinline__ void lds_barrier() {             // orders LDS only: 
 }
 
 // WM x WN wavefronts, each with a tile of FI x FJ fragments of 32 x 32.  PAIRED: the first half of a wavefront's column
-// fragments comes from the first product, the second half from the second.
-template <int WM, int WN, int FI, int FJ, bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
+// fragments comes from the first product, the second half from the second.  With two planes tiles that hold a marked row are left
+// out; with three and g.a_scale given, all others are.
+template <int PLANES, int WM, int WN, int FI, int FJ, bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
 __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Product<float> g) {
     constexpr int THREADS = WM * WN * 64, BM = WM * FI * 32, BN = WN * FJ * 32, HALF = PAIRED ? BN / 2 : BN;
-    typedef SplitShare<BM, A_ALONG, THREADS> AShare;
-    typedef SplitShare<BN, B_ALONG, THREADS> BShare;
-    constexpr unsigned A_BYTES = 3 * AShare::PLANE, BUFFER = A_BYTES + 3 * BShare::PLANE;
+    typedef SplitShare<PLANES, BM, A_ALONG, THREADS> AShare;
+    typedef SplitShare<PLANES, BN, B_ALONG, THREADS> BShare;
+    typedef Partial<PLANES> Part;
+    constexpr unsigned A_BYTES = PLANES * AShare::PLANE, BUFFER = A_BYTES + PLANES * BShare::PLANE;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];          // two buffers
     const unsigned tiles = (unsigned)(g.tiles_m * g.tiles_n), part = blockIdx.x / tiles;
     int tm, tn;
     own_tile(blockIdx.x - part * tiles, tiles, g.tiles_m, g.tiles_n, tm, tn);
     const int m0 = tm * BM, n0 = tn * HALF;
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, wm = wave / WN, wn = wave % WN;
+    // exponent of the tile's row r, column c (columns of a pair: the first product's, then the second's)
+    const auto row_exponent = [&](int r) { return g.a_scale[m0 + r < g.rows ? m0 + r : g.rows - 1]; };
+    const auto column_exponent = [&](int c) {
+        const int n = n0 + (PAIRED && c >= HALF ? c - HALF : c);
+        return g.b_scale[PAIRED && c >= HALF][n < g.cols ? n : g.cols - 1];
+    };
+    if (PLANES == 2 || g.a_scale) {
+        bool marked = false;
+        for (int r = t; r < BM; r += THREADS) marked |= row_exponent(r) == MARKED;
+        for (int c = t; c < BN; c += THREADS) marked |= column_exponent(c) == MARKED;
+        if ((__syncthreads_or(marked) != 0) != (PLANES == 3)) return;
+    }
     AShare a;
     BShare b;
-    a.place(g.A[0], g.lda, m0, g.rows, t, 0, nullptr);
-    b.place(g.B[0], g.ldb, n0, g.cols, t, PAIRED ? HALF : 0, g.B[1]);
+    a.place(g.A[0], g.lda, m0, g.rows, t, 0, nullptr, g.a_scale, nullptr);
+    b.place(g.B[0], g.ldb, n0, g.cols, t, PAIRED ? HALF : 0, g.B[1], g.b_scale[0], g.b_scale[1]);
     const int64_t a_shift = g.segments > 1 ? g.A[1] - g.A[0] : 0, b_shift = g.segments > 1 ? g.B[1] - g.B[0] : 0;
     // Whole slices of all segments first, g.steps_per_part of them per part; the last part also takes what is left of each segment.
     const int whole = g.inner / 16, all = whole * g.segments;
@@ -321,23 +466,21 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
     const auto column_block = [&](int j) { return PAIRED ? (j / (FJ / 2)) * (BN / 64) + wn * (FJ / 2) + j % (FJ / 2) : wn * FJ + j; };
     const unsigned mine = (unsigned)((lane >> 5) * 512 + (((lane & 31) ^ ((lane >> 5) * 8)) * 16));
     f32x16 acc[FI][FJ] = {};
-    const auto read_a = [&](const unsigned char* from, int i, bf16x8 (&f)[3]) {
+    const auto read_a = [&](const unsigned char* from, int i, u32x4 (&f)[PLANES]) {
 #pragma unroll
-        for (int k = 0; k < 3; k++) f[k] = *(const bf16x8*)(from + mine + k * AShare::PLANE + (wm * FI + i) * 1024);
+        for (int k = 0; k < PLANES; k++) f[k] = *(const u32x4*)(from + mine + k * AShare::PLANE + (wm * FI + i) * 1024);
     };
-    const auto read_b = [&](const unsigned char* from, bf16x8 (&f)[FJ][3]) {
+    const auto read_b = [&](const unsigned char* from, u32x4 (&f)[FJ][PLANES]) {
 #pragma unroll
-        for (int k = 0; k < 3; k++)
+        for (int k = 0; k < PLANES; k++)
 #pragma unroll
-            for (int j = 0; j < FJ; j++) f[j][k] = *(const bf16x8*)(from + mine + A_BYTES + k * BShare::PLANE + column_block(j) * 1024);
+            for (int j = 0; j < FJ; j++) f[j][k] = *(const u32x4*)(from + mine + A_BYTES + k * BShare::PLANE + column_block(j) * 1024);
     };
-    const auto multiply = [&](int i, const bf16x8 (&af)[3], const bf16x8 (&bf)[FJ][3]) {
-        constexpr int order[6][2] = {{0, 0}, {1, 0}, {2, 0}, {0, 1}, {1, 1}, {0, 2}};
+    const auto multiply = [&](int i, const u32x4 (&af)[PLANES], const u32x4 (&bf)[FJ][PLANES]) {
 #pragma unroll
-        for (int c = 0; c < 6; c++)
+        for (int c = 0; c < Part::N; c++)
 #pragma unroll
-            for (int j = 0; j < FJ; j++)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[order[c][0]], bf[j][order[c][1]], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < FJ; j++) acc[i][j] = Part::mma(af[Part::A[c]], bf[j][Part::B[c]], acc[i][j]);
     };
 
     if (first < last) {
@@ -350,7 +493,7 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
         a.store(lds, t); b.store(lds + A_BYTES, t);
         request_a(clamp(first + 1)); request_b(clamp(first + 1));
         lds_barrier();
-        bf16x8 bf[FJ][3], af[2][3];
+        u32x4 bf[FJ][PLANES], af[2][PLANES];
         read_b(lds, bf);
         read_a(lds, 0, af[0]);
         unsigned now = 0;
@@ -364,9 +507,9 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
                 if (i == 0) { a.store(next, t); request_a(clamp(s + 2)); }
                 if (i == (FI > 2 ? 1 : 0)) { b.store(next + A_BYTES, t); request_b(clamp(s + 2)); }
 #pragma unroll
-                for (int n = 0; n < 6 * FJ; n++) {
+                for (int n = 0; n < Part::N * FJ; n++) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);           // a matrix instruction,
-                    __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);           // vector arithmetic in its shadow,
+                    __builtin_amdgcn_sched_group_barrier(0x002, PLANES == 2 ? 6 : 4, 0);           // vector arithmetic in its shadow,
                     __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);           // an LDS read,
                     __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);           // an LDS write,
                     __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);           // a request to memory
@@ -374,19 +517,19 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
                 __builtin_amdgcn_sched_barrier(0);
             }
             lds_barrier();
-            bf16x8 bn[FJ][3], an[3];
+            u32x4 bn[FJ][PLANES], an[PLANES];
             read_a(next, 0, an);
             read_b(next, bn);
             multiply(FI - 1, af[(FI - 1) & 1], bf);
 #pragma unroll
-            for (int n = 0; n < 3 + 3 * FJ; n++) {
+            for (int n = 0; n < PLANES * (1 + FJ); n++) {
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
             // (without the empty statements the compiler moves these reads to the head of the loop, where nothing hides them)
 #pragma unroll
-            for (int k = 0; k < 3; k++) {
+            for (int k = 0; k < PLANES; k++) {
                 asm volatile("" : "+v"(an[k]));
                 af[0][k] = an[k];
 #pragma unroll
@@ -405,7 +548,7 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
             b.template load<false>(segment ? b_shift : 0, g.ldb, whole * 16, g.inner);
             a.store(lds, t); b.store(lds + A_BYTES, t);
             lds_barrier();
-            bf16x8 bf[FJ][3], af[3];
+            u32x4 bf[FJ][PLANES], af[PLANES];
             read_b(lds, bf);
 #pragma unroll
             for (int i = 0; i < FI; i++) { read_a(lds, i, af); multiply(i, af, bf); }
@@ -413,40 +556,52 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
         }
     }
 
+    // (two planes: the slices' memory takes the exponents of the tile's rows and columns; every row in it is finite, and so is every sum)
+    int* const exponents = (int*)lds;
     bool odd = false;
+    if constexpr (PLANES == 2) {
+        for (int r = t; r < BM; r += THREADS) exponents[r] = row_exponent(r);
+        for (int c = t; c < BN; c += THREADS) exponents[BM + c] = column_exponent(c);
+        lds_barrier();
+    } else {
 #pragma unroll
-    for (int i = 0; i < FI; i++)
+        for (int i = 0; i < FI; i++)
 #pragma unroll
-        for (int j = 0; j < FJ; j++)
+            for (int j = 0; j < FJ; j++)
 #pragma unroll
-            for (int v = 0; v < 16; v++) odd |= !(__builtin_fabsf(acc[i][j][v]) < INFINITY);
+                for (int v = 0; v < 16; v++) odd |= !(__builtin_fabsf(acc[i][j][v]) < INFINITY);
+    }
     // one fragment of the result (PAIRED: the same fragment of both products) to where it belongs.
     // Register v of lane l: row 8 (v / 4) + 4 (l / 32) + v % 4, column l % 32 of the fragment.
     const int64_t shift = (int64_t)part * g.part_stride;
-    const auto write = [&](int i, int j, const f32x16& x, const f32x16& y) {
-        const int n = n0 + (PAIRED ? wn * (FJ / 2) + j : wn * FJ + j) * 32 + (lane & 31);
+    const auto write = [&](int i, int j, const f32x16& xs, const f32x16& ys) {
+        const int c = (PAIRED ? wn * (FJ / 2) + j : wn * FJ + j) * 32 + (lane & 31), n = n0 + c;
+        const int x_exponent = PLANES == 2 ? exponents[BM + c] : 0, y_exponent = PLANES == 2 && PAIRED ? exponents[BM + HALF + c] : 0;
 #pragma unroll
         for (int v = 0; v < 16; v++) {
-            const int m = m0 + (wm * FI + i) * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
+            const int r = (wm * FI + i) * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3), m = m0 + r;
             if (m >= g.rows || n >= g.cols) continue;
             const int64_t at = (int64_t)m * g.cols + n + shift;
+            const float x = PLANES == 2 ? __builtin_ldexpf(xs[v], -(exponents[r] + x_exponent)) : xs[v];
+            const float y = !PAIRED ? 0.0f : PLANES == 2 ? __builtin_ldexpf(ys[v], -(exponents[r] + y_exponent)) : ys[v];
             if constexpr (PAIRED && EPI == GATED) {
-                g.out[0][at] = gated_fun(g.fun, x[v]) * y[v];
-                if (g.out[1]) { g.out[1][at] = x[v]; g.out[2][at] = y[v]; }
+                g.out[0][at] = gated_fun(g.fun, x) * y;
+                if (g.out[1]) { g.out[1][at] = x; g.out[2][at] = y; }
             } else {
-                g.out[0][at] = x[v];
-                if constexpr (PAIRED) g.out[1][at] = y[v];
+                g.out[0][at] = x;
+                if constexpr (PAIRED) g.out[1][at] = y;
             }
         }
     };
     constexpr int SHOWN = PAIRED ? FJ / 2 : FJ;             // fragments per row of the wavefront's tile, of one product
-    if (!__any(odd)) {
+    if (PLANES == 2 || !__any(odd)) {
 #pragma unroll
         for (int i = 0; i < FI; i++)
 #pragma unroll
             for (int j = 0; j < SHOWN; j++) write(i, j, acc[i][j], acc[i][PAIRED ? FJ / 2 + j : j]);
         return;
     }
+    if constexpr (PLANES == 3)
 #pragma unroll 1
     for (int f = 0; f < FI * SHOWN; f++) {
         const int i = f / SHOWN, j = f % SHOWN;
@@ -684,12 +839,18 @@ static uint64_t partial_elements(const Split& s, bool paired, int64_t rows, int6
 
 template <bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
 static void launch_tiles(Device* dev, const Product<float>& g, const Split& s, dim3 grid) {
-    const auto go = [&](auto kernel, int threads, unsigned lds) {
-        (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, dev->stream, g);
+    const auto go = [&](auto planes) {
+        constexpr int P = decltype(planes)::value;
+        const auto run = [&](auto kernel, int threads, unsigned edge) {
+            const unsigned lds = 2 * P * 2 * edge * 32;      // two buffers of both operands' planes
+            (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, dev->stream, g);
+        };
+        if (s.large) run(split_product_kernel<P, 2, 4, 4, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 512, 256);
+        else         run(split_product_kernel<P, 2, 2, 2, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 256, 128);
     };
-    if (s.large) go(split_product_kernel<2, 4, 4, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 512, 2 * 2 * 3 * 256 * 32);
-    else         go(split_product_kernel<2, 2, 2, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 256, 2 * 2 * 3 * 128 * 32);
+    if (g.a_scale) go(std::integral_constant<int, 2>());
+    go(std::integral_constant<int, 3>());                    // (with scales: the tiles that the launch before left out)
 }
 template <bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
 static void launch_tiles(Device* dev, const Product<double>& g, const Split&, dim3 grid) {
@@ -767,6 +928,20 @@ static int launch_few(Device* dev, Product<T> g, const FewPlan& f, bool along, T
     return NK_OK;
 }
 
+// Whether a product of that many multiply-adds takes two planes: they save half of its matrix instructions and cost two launches and
+// a read of the operands before it.
+template <typename T> static bool two_planes(int64_t rows, int64_t cols, int64_t inner) {
+    return sizeof(T) == 4 && rows > 64 && rows * cols * inner >= TWO_PLANES_FROM;
+}
+static void add_job(ScaleJobs& jobs, const float* p, const float* second, int64_t ld, int64_t count, int64_t length, bool along, int* out) {
+    jobs.job[jobs.n++] = {{p, second}, ld, (int)count, (int)length, along, out, (unsigned)(along ? (count + 7) / 8 : (count + 31) / 32)};
+}
+static void launch_scales(Device* dev, const ScaleJobs& jobs) {
+    unsigned blocks = 0;
+    for (int i = 0; i < jobs.n; i++) blocks += jobs.job[i].blocks;
+    hipLaunchKernelGGL(operand_scales_kernel, dim3(blocks), dim3(512), 0, dev->stream, jobs);
+}
+
 template <typename T>
 static int gated_forward(Device* dev, int fun, bool along, int64_t M, int64_t K, int64_t N, const T* X, const T* Wg, const T* Wu, T* H, T* gate, T* up) {
     Product<T> g{};
@@ -784,8 +959,18 @@ static int gated_forward(Device* dev, int fun, bool along, int64_t M, int64_t K,
         return NK_OK;
     }
     const Split s = plan<T>(dev, true, M, N, K, 1);
-    if (const uint64_t need = partial_elements(s, true, M, N))
-        if (int e = workspace(dev, need * sizeof(T), &ws)) return e;
+    const bool two = two_planes<T>(M, 2 * N, K);
+    const uint64_t parts_bytes = partial_elements(s, true, M, N) * sizeof(T), need = parts_bytes + (two ? (M + 2 * N) * sizeof(int) : 0);
+    if (need) if (int e = workspace(dev, need, &ws)) return e;
+    if constexpr (sizeof(T) == 4) if (two) {
+        int* const scales = (int*)((char*)ws + parts_bytes);
+        ScaleJobs jobs{};
+        add_job(jobs, X, nullptr, K, M, K, true, scales);
+        add_job(jobs, Wg, nullptr, g.ldb, N, K, along, scales + M);
+        add_job(jobs, Wu, nullptr, g.ldb, N, K, along, scales + M + N);
+        launch_scales(dev, jobs);
+        g.a_scale = scales; g.b_scale[0] = scales + M; g.b_scale[1] = scales + M + N;
+    }
     launch_product<T, true, GATED>(dev, g, s, true, along, (T*)ws);
     NK_HIP(hipGetLastError());
     set_path(s.parts > 1 ? "gated_tiles_split" : "gated_tiles");
@@ -799,25 +984,43 @@ static int gated_backward(Device* dev, int fun, bool along, int64_t M, int64_t K
     const Split sx = plan<T>(dev, false, M, K, N, 2), sw = plan<T>(dev, true, K, N, M, 1);
     const FewPlan few = few_plan<T>(dev, M, K, N);
     const uint64_t px = dX ? M <= 64 ? few_partial_elements(few, M, K) : partial_elements(sx, false, M, K) : 0, pw = dWg ? partial_elements(sw, true, K, N) : 0;
+    const bool two_x = dX && two_planes<T>(M, K, 2 * N), two_w = dWg && two_planes<T>(K, 2 * N, M) && M > 64;
+    const uint64_t scales_x = two_x ? M + K : 0, scales_w = two_w ? K + 2 * N : 0;
     void* ws = nullptr;
-    if (int e = workspace(dev, (2 * (uint64_t)n + (px > pw ? px : pw)) * sizeof(T), &ws)) return e;
+    if (int e = workspace(dev, (2 * (uint64_t)n + (px > pw ? px : pw)) * sizeof(T) + (scales_x + scales_w) * sizeof(int), &ws)) return e;
     T *const dg = (T*)ws, *const du = dg + n, *const partial = du + n;
     hipLaunchKernelGGL((gated_errors_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, dev->stream, fun, n, E, gate, up, dg, du);
+    Product<T> gx{}, gw{};
+    gx.A[0] = dg; gx.A[1] = du; gx.lda = N; gx.B[0] = Wg; gx.B[1] = Wu; gx.ldb = along ? K : N;      // (weights stored by row have neighbours along N)
+    gx.rows = (int)M; gx.cols = (int)K; gx.inner = (int)N; gx.segments = 2;
+    gx.out[0] = dX;
+    gw.A[0] = X; gw.lda = K; gw.B[0] = dg; gw.B[1] = du; gw.ldb = N;
+    gw.rows = (int)K; gw.cols = (int)N; gw.inner = (int)M; gw.segments = 1;
+    gw.out[0] = dWg; gw.out[1] = dWu;
+    if constexpr (sizeof(T) == 4) {
+        int* const scales = (int*)(partial + (px > pw ? px : pw));
+        if (two_x) {
+            ScaleJobs jobs{};
+            add_job(jobs, dg, du, N, M, N, true, scales);
+            add_job(jobs, Wg, Wu, gx.ldb, K, N, !along, scales + M);
+            launch_scales(dev, jobs);
+            gx.a_scale = scales; gx.b_scale[0] = scales + M;
+        }
+        if (two_w) {
+            int* const at = scales + scales_x;
+            ScaleJobs jobs{};
+            add_job(jobs, X, nullptr, K, K, M, false, at);
+            add_job(jobs, dg, nullptr, N, N, M, false, at + K);
+            add_job(jobs, du, nullptr, N, N, M, false, at + K + N);
+            launch_scales(dev, jobs);
+            gw.a_scale = at; gw.b_scale[0] = at + K; gw.b_scale[1] = at + K + N;
+        }
+    }
     if (dX) {
-        Product<T> g{};
-        g.A[0] = dg; g.A[1] = du; g.lda = N; g.B[0] = Wg; g.B[1] = Wu; g.ldb = along ? K : N;
-        g.rows = (int)M; g.cols = (int)K; g.inner = (int)N; g.segments = 2;
-        g.out[0] = dX;
-        if (M <= 64) { if (int e = launch_few<T, SUM>(dev, g, few, !along, partial)) return e; }
-        else launch_product<T, false, STORE>(dev, g, sx, true, !along, partial);      // (weights stored by row have neighbours along N)
+        if (M <= 64) { if (int e = launch_few<T, SUM>(dev, gx, few, !along, partial)) return e; }
+        else launch_product<T, false, STORE>(dev, gx, sx, true, !along, partial);
     }
-    if (dWg) {
-        Product<T> g{};
-        g.A[0] = X; g.lda = K; g.B[0] = dg; g.B[1] = du; g.ldb = N;
-        g.rows = (int)K; g.cols = (int)N; g.inner = (int)M; g.segments = 1;
-        g.out[0] = dWg; g.out[1] = dWu;
-        launch_product<T, true, STORE>(dev, g, sw, false, false, partial);
-    }
+    if (dWg) launch_product<T, true, STORE>(dev, gw, sw, false, false, partial);
     NK_HIP(hipGetLastError());
     set_path("gated_backward_tiles");
     return NK_OK;

@@ -543,3 +543,75 @@ def test_two_handles_of_the_device_do_not_mix(device):
         del b, theirs
     finally:
         other.dispose()
+
+
+# ---- products large enough for two half-precision planes -----------------------------------------------------------
+
+LARGE = [(1300, 1310, 1290), (1111, 2000, 1003), (4099, 500, 1100), (700, 3000, 1100)]
+
+
+def rows_of(device, x, wg, wu, along=False):
+    """gate and up of a product, straight from the device."""
+    M, N = x.shape[0], wg.shape[1]
+    gate, up = (device.allocate(np.float32, M * N) for _ in range(2))
+    put_w = (lambda w: put(device, np.ascontiguousarray(w.T)).T()) if along else (lambda w: put(device, w))
+    device.launch_gated_matmul("idy", put(device, np.zeros((M, N), np.float32)), put(device, x), put_w(wg), put_w(wu), gate, up)
+    return [device._read_all(d).reshape(M, N) for d in (gate, up)]
+
+
+@pytest.mark.parametrize("along", [False, True])
+@pytest.mark.parametrize("M,K,N", LARGE)
+def test_large_gated_products_and_gradients(device, along, M, K, N):
+    check_gated(device, np.float32, "silu", M, K, N, along)
+
+
+@pytest.mark.parametrize("along", [False, True])
+def test_large_gated_products_of_integers_are_exact(device, along):
+    """Integers of up to 11 bits are halves: every partial product and sum below 2^24 is exact."""
+    rng = np.random.default_rng(20)
+    M, K, N = 1301, 1307, 1299
+    x = rng.integers(-30, 31, (M, K)).astype(np.float32)
+    wg, wu = (rng.integers(-30, 31, (K, N)).astype(np.float32) for _ in range(2))
+    for got, w in zip(rows_of(device, x, wg, wu, along), (wg, wu)):
+        assert (got == x.astype(np.float64) @ w.astype(np.float64)).all()
+
+
+def test_large_gated_rows_of_any_magnitude_keep_their_digits(device):
+    """Rows and columns from 2^-100 to 2^100, zero rows and columns, and rows whose entries lie 2^30 apart (with and without a
+    counterpart): each result is as exact as its own terms allow."""
+    rng = np.random.default_rng(21)
+    M, K, N = 1200, 1400, 1310
+    x = (rng.standard_normal((M, K)) * 2.0 ** rng.integers(-50, 50, (M, 1))).astype(np.float32)
+    wg, wu = ((rng.standard_normal((K, N)) * 2.0 ** rng.integers(-50, 50, (1, N))).astype(np.float32) for _ in range(2))
+    x[5], wg[:, 7], wu[:, 1309] = 0, 0, 0
+    x[300:310, 100] *= 2.0 ** 30                            # one entry far above its row ...
+    wg[100], wu[100] = 0, 0                                 # ... that meets nothing
+    wg[200, 600:640] *= 2.0 ** 30
+    x[1199, :700] *= 2.0 ** -30                             # half a row far below the other half
+    for got, w in zip(rows_of(device, x, wg, wu), (wg, wu)):
+        X, W = x.astype(np.float64), w.astype(np.float64)
+        want = X @ W
+        over = np.abs(want) > np.finfo(np.float32).max       # (2^50 2^50 2^30: a few sums leave the type's range)
+        assert (got[over] == np.sign(want[over]) * np.inf).all()
+        within(got[~over], want[~over], (sum_roundings(K) * unit(np.float32) * (np.abs(X) @ np.abs(W)))[~over], "gate or up")
+
+
+def test_large_gated_infinities_and_nan(device):
+    rng = np.random.default_rng(22)
+    M, K, N = 1200, 1400, 1310
+    x, wg, wu = (rng.standard_normal(s).astype(np.float32) for s in ((M, K), (K, N), (K, N)))
+    x[0, 3], x[700, 4], x[M - 1, K - 1] = np.inf, np.nan, -np.inf
+    wg[7, 11], wu[8, N - 1] = np.inf, -np.inf
+    with np.errstate(all="ignore"):
+        for got, w in zip(rows_of(device, x, wg, wu), (wg, wu)):
+            X, W = x.astype(np.float64), w.astype(np.float64)
+            fine_x, fine_w = np.isfinite(X).all(1), np.isfinite(W).all(0)
+            want = np.where(np.isfinite(X), X, 0) @ np.where(np.isfinite(W), W, 0)
+            for i in np.flatnonzero(~fine_x):
+                want[i] = (X[i][:, None] * W).sum(0)
+            for j in np.flatnonzero(~fine_w):
+                want[:, j] = (X * W[:, j]).sum(1)
+            assert (np.isnan(got) == np.isnan(want)).all() and (np.where(np.isinf(want), got == want, True)).all()
+            ok = np.isfinite(want)
+            amount = np.abs(np.where(np.isfinite(X), X, 0)) @ np.abs(np.where(np.isfinite(W), W, 0))
+            within(got[ok], want[ok], sum_roundings(K) * unit(np.float32) * amount[ok], "finite ones")
