@@ -221,12 +221,12 @@ __device__ __forceinline__ void split_pair(float x, float y, unsigned (&p)[3]) {
         }
     }
 }
-// two scaled floats -> their two pairs of halves
-__device__ __forceinline__ void split_pair(float x, float y, unsigned (&p)[2]) {
-    const f16x2 high = {(_Float16)x, (_Float16)y};
-    const f16x2 low = {(_Float16)(x - (float)high[0]), (_Float16)(y - (float)high[1])};
+// two floats times a power of two (exact) -> their two pairs of halves; the rest is formed by a multiply-add that takes the half as it is
+__device__ __forceinline__ void split_pair(float x, float y, float by, unsigned (&p)[2]) {
+    const f16x2 high = __builtin_convertvector((f32x2{x * by, y * by}), f16x2);
+    const f32x2 rest = {__builtin_fmaf(x, by, -(float)high[0]), __builtin_fmaf(y, by, -(float)high[1])};
     p[0] = __builtin_bit_cast(unsigned, high);
-    p[1] = __builtin_bit_cast(unsigned, low);
+    p[1] = __builtin_bit_cast(unsigned, __builtin_convertvector(rest, f16x2));
 }
 template <int PLANES> struct Partial;
 template <> struct Partial<3> {
@@ -341,7 +341,7 @@ struct SplitShare {
     static constexpr int E = WIDTH * 16 / THREADS;          // elements per thread: 4 or 8
     static constexpr unsigned PLANE = WIDTH * 32;           // bytes
     static_assert(E == 4 || E == 8, "a thread moves one or two times four elements");
-    float v[E];
+    float v[2][E];                                          // two slices on their way
     const float* base[E / 4];                               // ALONG: the thread's rows; else: its column (base[0])
     float scale[E / 4];                                     // two planes: their powers of two
     int l_of;                                               // first l of the thread inside a slice
@@ -362,7 +362,7 @@ struct SplitShare {
         l_of = ALONG ? (t & 3) * 4 : __builtin_amdgcn_readfirstlane(t / WIDTH) * E;
     }
     // shift: from the first segment to this one.  WHOLE: all 16 l of the slice exist; else what lies past `inner` is zero.
-    template <bool WHOLE>
+    template <int SET, bool WHOLE>
     __device__ __forceinline__ void load(int64_t shift, int64_t ld, int l0, int inner) {
         const int l = l0 + l_of;
         if constexpr (ALONG) {
@@ -372,24 +372,25 @@ struct SplitShare {
                 if constexpr (WHOLE) {
                     const f32x4 q = *(const f32x4_any*)at;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[u * 4 + e] = q[e];
+                    for (int e = 0; e < 4; e++) v[SET][u * 4 + e] = q[e];
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[u * 4 + e] = l + e < inner ? at[e] : 0.0f;
+                    for (int e = 0; e < 4; e++) v[SET][u * 4 + e] = l + e < inner ? at[e] : 0.0f;
                 }
             }
         } else {
             const float* const at = base[0] + shift + (int64_t)l * ld;
 #pragma unroll
-            for (int e = 0; e < E; e++) v[e] = WHOLE || l + e < inner ? at[(int64_t)e * ld] : 0.0f;
+            for (int e = 0; e < E; e++) v[SET][e] = WHOLE || l + e < inner ? at[(int64_t)e * ld] : 0.0f;
         }
     }
+    template <int SET>
     __device__ __forceinline__ void store(unsigned char* lds, int t) const {
         unsigned p[E / 2][PLANES];
 #pragma unroll
         for (int e = 0; e < E / 2; e++) {
-            const float by = PLANES == 2 ? scale[ALONG ? e / 2 : 0] : 1.0f;
-            split_pair(PLANES == 2 ? v[2 * e] * by : v[2 * e], PLANES == 2 ? v[2 * e + 1] * by : v[2 * e + 1], p[e]);
+            if constexpr (PLANES == 2) split_pair(v[SET][2 * e], v[SET][2 * e + 1], scale[ALONG ? e / 2 : 0], p[e]);
+            else split_pair(v[SET][2 * e], v[SET][2 * e + 1], p[e]);
         }
         if constexpr (ALONG) {
             const int q = t & 3, high = q >> 1;
@@ -455,13 +456,13 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
     const int whole = g.inner / 16, all = whole * g.segments;
     const int first = (int)part * g.steps_per_part < all ? (int)part * g.steps_per_part : all;
     const int last = first + g.steps_per_part < all ? first + g.steps_per_part : all;
-    const auto request_a = [&](int s) {
+    const auto request_a = [&](auto set, int s) {
         const int segment = s >= whole;
-        a.template load<true>(segment ? a_shift : 0, g.lda, (s - segment * whole) * 16, g.inner);
+        a.template load<decltype(set)::value, true>(segment ? a_shift : 0, g.lda, (s - segment * whole) * 16, g.inner);
     };
-    const auto request_b = [&](int s) {
+    const auto request_b = [&](auto set, int s) {
         const int segment = s >= whole;
-        b.template load<true>(segment ? b_shift : 0, g.ldb, (s - segment * whole) * 16, g.inner);
+        b.template load<decltype(set)::value, true>(segment ? b_shift : 0, g.ldb, (s - segment * whole) * 16, g.inner);
     };
     const auto column_block = [&](int j) { return PAIRED ? (j / (FJ / 2)) * (BN / 64) + wn * (FJ / 2) + j % (FJ / 2) : wn * FJ + j; };
     const unsigned mine = (unsigned)((lane >> 5) * 512 + (((lane & 31) ^ ((lane >> 5) * 8)) * 16));
@@ -484,32 +485,42 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
     };
 
     if (first < last) {
-        // The loop is one block without a branch.  Slice s is in LDS and the first fragments of it in registers; slice s + 1 is in
-        // registers as floats and goes to LDS between the matrix instructions, slice s + 2 is requested as soon as its registers are
-        // free (past the end: the last slice once more).  The barrier stands before the last row of fragments: behind it, while those
-        // are multiplied, the first fragments of the next slice are read.
+        // A slice is one block without a branch.  Slice s is in LDS and the first fragments of it in registers; slices s + 1 and s + 2 are in
+        // registers as floats or on their way (one slice takes 1.5 us, less than a loaded memory's answer: with slice s + 1 alone
+        // on its way 4096^3 took 770 us).  s + 1 goes to LDS between the matrix instructions and its registers are asked for s + 3 (past
+        // the end: the last slice once more).  The barrier stands before the last rows of fragments: behind it, while those are multiplied,
+        // the first fragments of the next slice are read.
+        typedef std::integral_constant<int, 0> Even;
+        typedef std::integral_constant<int, 1> Odd;
         const auto clamp = [&](int s) { return s < last ? s : last - 1; };
-        request_a(first); request_b(first);
-        a.store(lds, t); b.store(lds + A_BYTES, t);
-        request_a(clamp(first + 1)); request_b(clamp(first + 1));
+        request_a(Even(), first); request_b(Even(), first);
+        request_a(Odd(), clamp(first + 1)); request_b(Odd(), clamp(first + 1));
+        a.template store<0>(lds, t); b.template store<0>(lds + A_BYTES, t);
+        request_a(Even(), clamp(first + 2)); request_b(Even(), clamp(first + 2));
         lds_barrier();
-        u32x4 bf[FJ][PLANES], af[2][PLANES];
+        // rows of fragments multiplied before the barrier; the others' fragments wait in registers
+        constexpr int BEFORE = PLANES == 2 ? FI / 2 : FI - 1, HELD = FI - BEFORE + 1;
+        u32x4 bf[FJ][PLANES], af[HELD][PLANES];
         read_b(lds, bf);
         read_a(lds, 0, af[0]);
-        unsigned now = 0;
-        for (int s = first; s < last; s++) {
-            const unsigned char* const cur = lds + now;
-            unsigned char* const next = lds + (BUFFER - now);
+        const auto slice = [&](auto parity, int s) {
+            constexpr int P = decltype(parity)::value;
+            std::integral_constant<int, 1 - P> other;
+            const unsigned char* const cur = lds + P * BUFFER;
+            unsigned char* const next = lds + (1 - P) * BUFFER;
 #pragma unroll
-            for (int i = 0; i < FI - 1; i++) {
-                read_a(cur, i + 1, af[(i + 1) & 1]);
-                multiply(i, af[i & 1], bf);
-                if (i == 0) { a.store(next, t); request_a(clamp(s + 2)); }
-                if (i == (FI > 2 ? 1 : 0)) { b.store(next + A_BYTES, t); request_b(clamp(s + 2)); }
+            for (int i = 0; i < BEFORE; i++) {
+                if (i + 1 < BEFORE) read_a(cur, i + 1, af[(i + 1) % HELD]);
+                else
+#pragma unroll
+                    for (int r = BEFORE; r < FI; r++) read_a(cur, r, af[r % HELD]);
+                multiply(i, af[i % HELD], bf);
+                if (i == 0) { a.template store<1 - P>(next, t); request_a(other, clamp(s + 3)); }
+                if (i == (BEFORE > 1 ? 1 : 0)) { b.template store<1 - P>(next + A_BYTES, t); request_b(other, clamp(s + 3)); }
 #pragma unroll
                 for (int n = 0; n < Part::N * FJ; n++) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);           // a matrix instruction,
-                    __builtin_amdgcn_sched_group_barrier(0x002, PLANES == 2 ? 6 : 4, 0);           // vector arithmetic in its shadow,
+                    __builtin_amdgcn_sched_group_barrier(0x002, PLANES == 2 ? 8 : 4, 0);           // vector arithmetic in its shadow,
                     __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);           // an LDS read,
                     __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);           // an LDS write,
                     __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);           // a request to memory
@@ -520,14 +531,15 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
             u32x4 bn[FJ][PLANES], an[PLANES];
             read_a(next, 0, an);
             read_b(next, bn);
-            multiply(FI - 1, af[(FI - 1) & 1], bf);
+#pragma unroll
+            for (int i = BEFORE; i < FI; i++) multiply(i, af[i % HELD], bf);
 #pragma unroll
             for (int n = 0; n < PLANES * (1 + FJ); n++) {
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
-            // (without the empty statements the compiler moves these reads to the head of the loop, where nothing hides them)
+            // (without the empty statements the compiler moves these reads to the next slice, where nothing hides them)
 #pragma unroll
             for (int k = 0; k < PLANES; k++) {
                 asm volatile("" : "+v"(an[k]));
@@ -538,15 +550,20 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
                     bf[j][k] = bn[j][k];
                 }
             }
-            now = BUFFER - now;
+        };
+        int s = first;
+        for (; s + 1 < last; s += 2) {
+            slice(Even(), s);
+            slice(Odd(), s + 1);
         }
+        if (s < last) slice(Even(), s);
         lds_barrier();
     }
     if (g.inner % 16 != 0 && last == all) {
         for (int segment = 0; segment < g.segments; segment++) {
-            a.template load<false>(segment ? a_shift : 0, g.lda, whole * 16, g.inner);
-            b.template load<false>(segment ? b_shift : 0, g.ldb, whole * 16, g.inner);
-            a.store(lds, t); b.store(lds + A_BYTES, t);
+            a.template load<0, false>(segment ? a_shift : 0, g.lda, whole * 16, g.inner);
+            b.template load<0, false>(segment ? b_shift : 0, g.ldb, whole * 16, g.inner);
+            a.template store<0>(lds, t); b.template store<0>(lds + A_BYTES, t);
             lds_barrier();
             u32x4 bf[FJ][PLANES], af[PLANES];
             read_b(lds, bf);
