@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256) void product_kernel(const Product<T> g) {
 // So a launch before finds, for every row of A and of B, the power of two that brings its largest magnitude below
 // 2^15; what is 2^-16 of that or more keeps all its bits, and smaller numbers are off by at most 2^-40 of the largest.
 // A row where that could show -- more than a quarter of its 64 stretches hold nothing beyond 2^-16 of the largest (and are not all
-// zero), or an infinity or NaN -- is marked, and tiles with a marked row are left to a launch with three planes.
+// zero), or an infinity or NaN -- is marked, and tiles with a marked row take three planes.
 constexpr int64_t TWO_PLANES_FROM = (int64_t)1 << 32;        // multiply-adds
 constexpr int MARKED = 1 << 30;                              // in place of a row's exponent
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -420,20 +420,14 @@ __device__ __forceinline__ void lds_barrier() {             // orders LDS only: 
 }
 
 // WM x WN wavefronts, each with a tile of FI x FJ fragments of 32 x 32.  PAIRED: the first half of a wavefront's column
-// fragments comes from the first product, the second half from the second.  With two planes tiles that hold a marked row are left
-// out; with three and g.a_scale given, all others are.
+// fragments comes from the first product, the second half from the second.
 template <int PLANES, int WM, int WN, int FI, int FJ, bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
-__global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Product<float> g) {
+__device__ __forceinline__ void split_product_tile(const Product<float>& g, unsigned char* lds, unsigned part, int m0, int n0) {
     constexpr int THREADS = WM * WN * 64, BM = WM * FI * 32, BN = WN * FJ * 32, HALF = PAIRED ? BN / 2 : BN;
     typedef SplitShare<PLANES, BM, A_ALONG, THREADS> AShare;
     typedef SplitShare<PLANES, BN, B_ALONG, THREADS> BShare;
     typedef Partial<PLANES> Part;
     constexpr unsigned A_BYTES = PLANES * AShare::PLANE, BUFFER = A_BYTES + PLANES * BShare::PLANE;
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];          // two buffers
-    const unsigned tiles = (unsigned)(g.tiles_m * g.tiles_n), part = blockIdx.x / tiles;
-    int tm, tn;
-    own_tile(blockIdx.x - part * tiles, tiles, g.tiles_m, g.tiles_n, tm, tn);
-    const int m0 = tm * BM, n0 = tn * HALF;
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, wm = wave / WN, wn = wave % WN;
     // exponent of the tile's row r, column c (columns of a pair: the first product's, then the second's)
     const auto row_exponent = [&](int r) { return g.a_scale[m0 + r < g.rows ? m0 + r : g.rows - 1]; };
@@ -441,12 +435,6 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
         const int n = n0 + (PAIRED && c >= HALF ? c - HALF : c);
         return g.b_scale[PAIRED && c >= HALF][n < g.cols ? n : g.cols - 1];
     };
-    if (PLANES == 2 || g.a_scale) {
-        bool marked = false;
-        for (int r = t; r < BM; r += THREADS) marked |= row_exponent(r) == MARKED;
-        for (int c = t; c < BN; c += THREADS) marked |= column_exponent(c) == MARKED;
-        if ((__syncthreads_or(marked) != 0) != (PLANES == 3)) return;
-    }
     AShare a;
     BShare b;
     a.place(g.A[0], g.lda, m0, g.rows, t, 0, nullptr, g.a_scale, nullptr);
@@ -649,6 +637,30 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
     }
 }
 
+// SCALED: two planes, or three where the tile holds a marked row.
+template <bool SCALED, int WM, int WN, int FI, int FJ, bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
+__global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Product<float> g) {
+    constexpr int THREADS = WM * WN * 64, BM = WM * FI * 32, BN = WN * FJ * 32, HALF = PAIRED ? BN / 2 : BN;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];          // two buffers of both operands' planes
+    const unsigned tiles = (unsigned)(g.tiles_m * g.tiles_n), part = blockIdx.x / tiles;
+    int tm, tn;
+    own_tile(blockIdx.x - part * tiles, tiles, g.tiles_m, g.tiles_n, tm, tn);
+    const int m0 = tm * BM, n0 = tn * HALF;
+    if constexpr (SCALED) {
+        bool marked = false;
+        for (int r = threadIdx.x; r < BM; r += THREADS) marked |= g.a_scale[m0 + r < g.rows ? m0 + r : g.rows - 1] == MARKED;
+        for (int c = threadIdx.x; c < BN; c += THREADS) {
+            const int n = n0 + (c >= HALF ? c - HALF : c);
+            marked |= g.b_scale[c >= HALF][n < g.cols ? n : g.cols - 1] == MARKED;
+        }
+        if (__syncthreads_or(marked) == 0) {
+            split_product_tile<2, WM, WN, FI, FJ, A_ALONG, B_ALONG, PAIRED, EPI>(g, lds, part, m0, n0);
+            return;
+        }
+    }
+    split_product_tile<3, WM, WN, FI, FJ, A_ALONG, B_ALONG, PAIRED, EPI>(g, lds, part, m0, n0);
+}
+
 // ---- few rows ----------------------------------------------------------------------------------------------------------
 // Up to 64 rows the weights' bytes bound the products, so they go from memory straight into the registers of the matrix
 // instructions (16 x 16 x 4, of the element type itself), each element once.  A wavefront owns 16 CW columns of both products and
@@ -796,37 +808,70 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const Product<T> g
 }
 
 // ---- parts of the contraction, added in order -----------------------------------------------------------------------
-// partial: [parts][halves][n]; halves 2: the pair of products
+// partial: [parts][halves][n]; halves 2: the pair of products.  Four elements a thread.
 template <typename T, bool PAIRED, int EPI>
 __global__ __launch_bounds__(256) void product_join_kernel(const T* __restrict__ partial, int parts, int64_t n, int fun, T* out0, T* out1, T* out2) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    typedef T V __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
     constexpr int HALVES = PAIRED ? 2 : 1;
-    T x = partial[i], y = PAIRED ? partial[n + i] : T(0);
-    for (int p = 1; p < parts; p++) {
-        x += partial[(int64_t)p * HALVES * n + i];
-        if (PAIRED) y += partial[((int64_t)p * HALVES + 1) * n + i];
+    const auto finish = [&](int64_t at, T x, T y) {
+        if constexpr (EPI == GATED) {
+            out0[at] = gated_fun(fun, x) * y;
+            if (out1) { out1[at] = x; out2[at] = y; }
+        } else if constexpr (EPI == SUM) out0[at] = x + y;
+        else {
+            out0[at] = x;
+            if (PAIRED) out1[at] = y;
+        }
+    };
+    if (i + 4 <= n) {
+        V x = *(const V*)(partial + i), y = x;
+        if (PAIRED) y = *(const V*)(partial + n + i);
+#pragma unroll 4
+        for (int p = 1; p < parts; p++) {
+            x += *(const V*)(partial + (int64_t)p * HALVES * n + i);
+            if (PAIRED) y += *(const V*)(partial + ((int64_t)p * HALVES + 1) * n + i);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) finish(i + e, x[e], y[e]);
+        return;
     }
-    if constexpr (EPI == GATED) {
-        out0[i] = gated_fun(fun, x) * y;
-        if (out1) { out1[i] = x; out2[i] = y; }
-    } else if constexpr (EPI == SUM) out0[i] = x + y;
-    else {
-        out0[i] = x;
-        if (PAIRED) out1[i] = y;
+    for (int64_t at = i; at < n; at++) {
+        T x = partial[at], y = PAIRED ? partial[n + at] : T(0);
+        for (int p = 1; p < parts; p++) {
+            x += partial[(int64_t)p * HALVES * n + at];
+            if (PAIRED) y += partial[((int64_t)p * HALVES + 1) * n + at];
+        }
+        finish(at, x, y);
     }
 }
 
-// dg = E up f'(gate), du = E f(gate)
+// dg = E up f'(gate), du = E f(gate): five numbers through memory per element, four elements a thread
 template <typename T>
 __global__ __launch_bounds__(256) void gated_errors_kernel(int fun, int64_t n, const T* __restrict__ error, const T* __restrict__ gate, const T* __restrict__ up,
                                                            T* __restrict__ d_gate, T* __restrict__ d_up) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    typedef T V __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
     T f, slope;
-    gated_fun_and_slope(fun, gate[i], f, slope);
-    d_gate[i] = error[i] * up[i] * slope;
-    d_up[i] = error[i] * f;
+    if (i + 4 <= n) {
+        const V e = *(const V*)(error + i), g = *(const V*)(gate + i), u = *(const V*)(up + i);
+        V dg, du;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            gated_fun_and_slope(fun, g[k], f, slope);
+            dg[k] = e[k] * u[k] * slope;
+            du[k] = e[k] * f;
+        }
+        *(V*)(d_gate + i) = dg;
+        *(V*)(d_up + i) = du;
+    } else
+        for (int64_t at = i; at < n; at++) {
+            gated_fun_and_slope(fun, gate[at], f, slope);
+            d_gate[at] = error[at] * up[at] * slope;
+            d_up[at] = error[at] * f;
+        }
 }
 
 // ---- plans ---------------------------------------------------------------------------------------------------------------
@@ -856,18 +901,17 @@ static uint64_t partial_elements(const Split& s, bool paired, int64_t rows, int6
 
 template <bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
 static void launch_tiles(Device* dev, const Product<float>& g, const Split& s, dim3 grid) {
-    const auto go = [&](auto planes) {
-        constexpr int P = decltype(planes)::value;
-        const auto run = [&](auto kernel, int threads, unsigned edge) {
-            const unsigned lds = 2 * P * 2 * edge * 32;      // two buffers of both operands' planes
-            (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-            hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, dev->stream, g);
-        };
-        if (s.large) run(split_product_kernel<P, 2, 4, 4, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 512, 256);
-        else         run(split_product_kernel<P, 2, 2, 2, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 256, 128);
+    const auto run = [&](auto kernel, int threads, unsigned edge) {
+        const unsigned lds = 2 * 3 * 2 * edge * 32;          // two buffers of three planes of both operands
+        (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, dev->stream, g);
     };
-    if (g.a_scale) go(std::integral_constant<int, 2>());
-    go(std::integral_constant<int, 3>());                    // (with scales: the tiles that the launch before left out)
+    const auto go = [&](auto scaled) {
+        constexpr bool S = decltype(scaled)::value;
+        if (s.large) run(split_product_kernel<S, 2, 4, 4, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 512, 256);
+        else         run(split_product_kernel<S, 2, 2, 2, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 256, 128);
+    };
+    if (g.a_scale) go(std::true_type()); else go(std::false_type());
 }
 template <bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
 static void launch_tiles(Device* dev, const Product<double>& g, const Split&, dim3 grid) {
@@ -891,7 +935,7 @@ static void launch_product(Device* dev, Product<T> g, const Split& s, bool a_alo
     g.out[0] = partial; g.out[1] = partial + n; g.out[2] = nullptr;
     g.part_stride = n * (PAIRED ? 2 : 1);
     go(std::integral_constant<int, STORE>());
-    hipLaunchKernelGGL((product_join_kernel<T, PAIRED, EPI>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, dev->stream, partial, s.parts, n, g.fun, out[0], out[1], out[2]);
+    hipLaunchKernelGGL((product_join_kernel<T, PAIRED, EPI>), dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, dev->stream, partial, s.parts, n, g.fun, out[0], out[1], out[2]);
 }
 
 // The products of up to 64 rows.  one_a: both products have the same A (GATED), else each has its own (SUM).
@@ -939,7 +983,7 @@ static int launch_few(Device* dev, Product<T> g, const FewPlan& f, bool along, T
         // (with parts the two products of a GATED call still share their A, which STORE does not know: A[1] = A[0])
         g.A[1] = g.A[1] ? g.A[1] : g.A[0];
         rows(std::integral_constant<int, STORE>());
-        hipLaunchKernelGGL((product_join_kernel<T, true, EPI>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, dev->stream, partial, f.parts, n, g.fun, out[0], out[1], out[2]);
+        hipLaunchKernelGGL((product_join_kernel<T, true, EPI>), dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, dev->stream, partial, f.parts, n, g.fun, out[0], out[1], out[2]);
     }
     NK_HIP(refused);
     return NK_OK;
@@ -1006,7 +1050,7 @@ static int gated_backward(Device* dev, int fun, bool along, int64_t M, int64_t K
     void* ws = nullptr;
     if (int e = workspace(dev, (2 * (uint64_t)n + (px > pw ? px : pw)) * sizeof(T) + (scales_x + scales_w) * sizeof(int), &ws)) return e;
     T *const dg = (T*)ws, *const du = dg + n, *const partial = du + n;
-    hipLaunchKernelGGL((gated_errors_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, dev->stream, fun, n, E, gate, up, dg, du);
+    hipLaunchKernelGGL((gated_errors_kernel<T>), dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, dev->stream, fun, n, E, gate, up, dg, du);
     Product<T> gx{}, gw{};
     gx.A[0] = dg; gx.A[1] = du; gx.lda = N; gx.B[0] = Wg; gx.B[1] = Wu; gx.ldb = along ? K : N;      // (weights stored by row have neighbours along N)
     gx.rows = (int)M; gx.cols = (int)K; gx.inner = (int)N; gx.segments = 2;
