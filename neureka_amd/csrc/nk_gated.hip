@@ -664,29 +664,47 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
 // ---- few rows ----------------------------------------------------------------------------------------------------------
 // Up to 64 rows the weights' bytes bound the products, so they go from memory straight into the registers of the matrix
 // instructions (16 x 16 x 4, of the element type itself), each element once.  A wavefront owns 16 CW columns of both products and
-// RT x 16 rows; the block's WAVES wavefronts share the contraction in chunks of KC, chunk after chunk in turn, and add their sums
-// through LDS in order.  Inside a chunk quarter q of a wavefront takes l from V q on, so that a lane's V values of A (and of
-// weights stored along l) are one 16-byte load.
-template <typename T, int RT, int CW, int WAVES, bool ALONG, int EPI>
-__global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const Product<T> g) {
+// RT x 16 rows; the block's wavefronts share the contraction, U chunks of KC at a time in turn, and add their sums through LDS
+// in order.  Inside a chunk quarter q of a wavefront takes l from V q on, so that a lane's V values of A (and of weights stored
+// along l) are one 16-byte load.
+//
+// What the memory delivers depends on how the requests lie (4096 x 4096 twice in floats, 134 MB; reads alone): 64 bytes of a row per
+// wavefront and 256 blocks 32 us, 128 bytes and 256 blocks 25, 128 bytes and 128 blocks 34.  So a wavefront reads 128 bytes of a
+// row of weights, and where that leaves fewer blocks than units, g.parts blocks share a group of columns: each adds its sums
+// to memory, and the one that arrives last adds them all, part by part.  Weights stored along l are 128 bytes per column
+// (U chunks); there every group starts at another place of the contraction, because groups that walk in step
+// meet in the same memory channels (33 us in step, 28 apart).
+//
+// The shared sums are written and read by atomic accesses of the whole device, which pass the caches of the eight dies one
+// by one; fences would write back and drop those caches whole (84 us instead of 27 for the call above).  What orders them: a wavefront
+// waits for its stores before the block's barrier, behind which one thread announces the block's arrival.
+template <typename Acc, typename T>
+__device__ __forceinline__ void put_shared(T* at, const Acc& x) {
+#pragma unroll
+    for (int v = 0; v < 4; v++) __hip_atomic_store(at + v, x[v], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename Acc, typename T>
+__device__ __forceinline__ Acc get_shared(const T* at) {
+    Acc x;
+#pragma unroll
+    for (int v = 0; v < 4; v++) x[v] = __hip_atomic_load(at + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return x;
+}
+template <typename T, int RT, int CW, bool ALONG, int EPI>
+__global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int parts, T* partial, unsigned* arrived) {
     typedef Quad<T> Q;
     typedef typename Q::Acc Acc;
-    constexpr int V = 16 / sizeof(T), KC = 4 * V, U = RT > 2 ? 1 : 2, NA = EPI == GATED ? 1 : 2;      // U chunks are loaded at a time
+    constexpr int WAVES = 8, V = 16 / sizeof(T), KC = 4 * V, U = RT > 2 && !ALONG ? 1 : 2, NA = EPI == GATED ? 1 : 2, FRAGMENTS = RT * CW;
     typedef T VecV __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+    typedef T VecC __attribute__((ext_vector_type(CW), aligned(sizeof(T))));
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, c = lane & 15, q = lane >> 4;
-    const unsigned groups = (unsigned)g.tiles_n, part = blockIdx.x / groups;
-    int none, group;
-    own_tile(blockIdx.x - part * groups, groups, 1, g.tiles_n, none, group);
-    const int n0 = group * 16 * CW;
-    const T *brow[2][CW], *arow[NA][RT];                    // ALONG: the lane's CW columns; else brow[.][0]: column n0 + c CW
+    const int part = blockIdx.x / (unsigned)g.tiles_n, group = blockIdx.x - (unsigned)part * (unsigned)g.tiles_n;
+    // the lane's CW neighbouring columns (moved back where they would pass the last one; what it shares with others it does not store)
+    const int own = group * 16 * CW + c * CW, n0 = own + CW <= g.cols ? own : g.cols - CW;
+    const T *brow[2], *arow[NA][RT];
 #pragma unroll
-    for (int p = 0; p < 2; p++)
-#pragma unroll
-        for (int j = 0; j < CW; j++) {
-            const int n = ALONG ? n0 + j * 16 + c : n0 + c * CW + j;
-            brow[p][j] = g.B[p] + (int64_t)(n < g.cols ? n : g.cols - 1) * (ALONG ? g.ldb : 1);
-        }
+    for (int p = 0; p < 2; p++) brow[p] = g.B[p] + (int64_t)n0 * (ALONG ? g.ldb : 1);
 #pragma unroll
     for (int p = 0; p < NA; p++)
 #pragma unroll
@@ -703,15 +721,17 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const Product<T> g
             if constexpr (ALONG) {
 #pragma unroll
                 for (int j = 0; j < CW; j++) {
-                    const VecV w = *(const VecV*)(brow[p][j] + l);
+                    const VecV w = *(const VecV*)(brow[p] + j * g.ldb + l);
 #pragma unroll
                     for (int s = 0; s < V; s++) k.b[p][j][s] = w[s];
                 }
             } else
 #pragma unroll
-                for (int s = 0; s < V; s++)
+                for (int s = 0; s < V; s++) {
+                    const VecC w = *(const VecC*)(brow[p] + (l + s) * g.ldb);
 #pragma unroll
-                    for (int j = 0; j < CW; j++) k.b[p][j][s] = brow[p][j][(l + s) * g.ldb];
+                    for (int j = 0; j < CW; j++) k.b[p][j][s] = w[j];
+                }
         }
 #pragma unroll
         for (int p = 0; p < NA; p++)
@@ -730,7 +750,7 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const Product<T> g
 #pragma unroll
             for (int p = 0; p < 2; p++)
 #pragma unroll
-                for (int j = 0; j < CW; j++) k.b[p][j][s] = in ? brow[p][j][(l + s) * (ALONG ? 1 : g.ldb)] : T(0);
+                for (int j = 0; j < CW; j++) k.b[p][j][s] = in ? brow[p][ALONG ? j * g.ldb + l + s : (l + s) * g.ldb + j] : T(0);
 #pragma unroll
             for (int p = 0; p < NA; p++)
 #pragma unroll
@@ -747,19 +767,24 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const Product<T> g
 #pragma unroll
                     for (int j = 0; j < CW; j++) acc[p][r][j] = Q::mma(k.a[NA == 1 ? 0 : p][r][s], k.b[p][j][s], acc[p][r][j]);
     };
-    // whole chunks first + wave, first + wave + WAVES, ... below last; what is left over belongs to the last part's first wavefront
-    const int whole = g.inner / KC, first = (int)part * g.steps_per_part < whole ? (int)part * g.steps_per_part : whole;
+    // The part's whole chunks, U at a time: wavefront w takes units w, w + WAVES, ...  What is left of the part, and the contraction's
+    // last, partial chunk, belong to the last wavefront.
+    const int whole = g.inner / KC, first = part * g.steps_per_part < whole ? part * g.steps_per_part : whole;
     const int last = first + g.steps_per_part < whole ? first + g.steps_per_part : whole;
-    const int mine = last - first - wave > 0 ? (last - first - wave + WAVES - 1) / WAVES : 0;
-    const auto at = [&](int i) { return (int64_t)(first + wave + i * WAVES) * KC; };
-    int i = 0;
-    if (mine >= U) {
+    const int units = (last - first) / U, mine = units > wave ? (units - wave + WAVES - 1) / WAVES : 0;
+    const int turn = ALONG && units > 0 ? (int)((unsigned)group * 17u % (unsigned)units) : 0;
+    const auto at = [&](int i) {
+        int unit = wave + i * WAVES + turn;
+        if (ALONG) unit -= unit >= units ? units : 0;
+        return (int64_t)(first + unit * U) * KC;
+    };
+    if (mine > 0) {
         Chunk now[U], next[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) load(now[u], at(u));
-        for (; i + 2 * U <= mine; i += U) {
+        for (int u = 0; u < U; u++) load(now[u], at(0) + u * KC);
+        for (int i = 1; i < mine; i++) {
 #pragma unroll
-            for (int u = 0; u < U; u++) load(next[u], at(i + U + u));
+            for (int u = 0; u < U; u++) load(next[u], at(i) + u * KC);
             __builtin_amdgcn_sched_barrier(0);               // the requests go out before the products of the chunks that are here
 #pragma unroll
             for (int u = 0; u < U; u++) multiply(now[u]);
@@ -768,15 +793,15 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const Product<T> g
         }
 #pragma unroll
         for (int u = 0; u < U; u++) multiply(now[u]);
-        i += U;
     }
-    Chunk one;
-    for (; i < mine; i++) { load(one, at(i)); multiply(one); }
-    if (wave == 0 && last == whole && g.inner % KC != 0) { load_rest(one, (int64_t)whole * KC); multiply(one); }
+    if (wave == WAVES - 1) {
+        Chunk one;
+        for (int k = first + units * U; k < last; k++) { load(one, (int64_t)k * KC); multiply(one); }
+        if (last == whole && part == parts - 1 && g.inner % KC != 0) { load_rest(one, (int64_t)whole * KC); multiply(one); }
+    }
 
     // the wavefronts' sums: [wave][product][row tile][column fragment][lane], a fragment's four values at a time
     Acc* const sums = (Acc*)lds;
-    constexpr int FRAGMENTS = RT * CW;
 #pragma unroll
     for (int p = 0; p < 2; p++)
 #pragma unroll
@@ -784,25 +809,48 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(const Product<T> g
 #pragma unroll
             for (int j = 0; j < CW; j++) sums[((wave * 2 + p) * FRAGMENTS + r * CW + j) * 64 + lane] = acc[p][r][j];
     __syncthreads();
-    for (int f = wave; f < FRAGMENTS; f += WAVES) {
-        Acc x = sums[f * 64 + lane], y = sums[(FRAGMENTS + f) * 64 + lane];
+    const auto total = [&](int f, int p) {
+        Acc x = sums[(p * FRAGMENTS + f) * 64 + lane];
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) {
-            x += sums[((w * 2) * FRAGMENTS + f) * 64 + lane];
-            y += sums[((w * 2 + 1) * FRAGMENTS + f) * 64 + lane];
+        for (int w = 1; w < WAVES; w++) x += sums[((w * 2 + p) * FRAGMENTS + f) * 64 + lane];
+        return x;
+    };
+    T* const shared = partial + ((int64_t)group * (2 * FRAGMENTS * 64) + lane) * 4;          // part after part a whole result apart
+    const int64_t apart = (int64_t)g.tiles_n * (2 * FRAGMENTS * 64) * 4;
+    if (parts > 1) {
+        for (int f = wave; f < 2 * FRAGMENTS; f += WAVES) put_shared(shared + part * apart + f * 256, total(f % FRAGMENTS, f / FRAGMENTS));
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wavefront's sums have arrived
+        __syncthreads();
+        unsigned* const order = (unsigned*)lds;
+        if (t == 0) {
+            const unsigned n = __hip_atomic_fetch_add(arrived + group, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (n == (unsigned)parts - 1) __hip_atomic_store(arrived + group, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            *order = n;
         }
-        const int r = f / CW, j = f % CW, n = ALONG ? n0 + j * 16 + c : n0 + c * CW + j;
-        if (n >= g.cols) continue;
+        __syncthreads();
+        if (*order != (unsigned)parts - 1) return;
+    }
+    for (int f = wave; f < FRAGMENTS; f += WAVES) {
+        Acc x, y;
+        if (parts > 1) {
+            x = get_shared<Acc>(shared + f * 256);
+            y = get_shared<Acc>(shared + (FRAGMENTS + f) * 256);
+            for (int k = 1; k < parts; k++) {
+                x += get_shared<Acc>(shared + k * apart + f * 256);
+                y += get_shared<Acc>(shared + k * apart + (FRAGMENTS + f) * 256);
+            }
+        } else { x = total(f, 0); y = total(f, 1); }
+        const int r = f / CW, n = n0 + f % CW;
+        if (n < own || n >= g.cols) continue;
 #pragma unroll
         for (int v = 0; v < 4; v++) {
             const int m = r * 16 + Q::row(lane, v);
             if (m >= g.rows) continue;
-            const int64_t o = (int64_t)m * g.cols + n + (int64_t)part * g.part_stride;
+            const int64_t o = (int64_t)m * g.cols + n;
             if constexpr (EPI == GATED) {
                 g.out[0][o] = gated_fun(g.fun, x[v]) * y[v];
                 if (g.out[1]) { g.out[1][o] = x[v]; g.out[2][o] = y[v]; }
-            } else if constexpr (EPI == SUM) g.out[0][o] = x[v] + y[v];
-            else { g.out[0][o] = x[v]; g.out[1][o] = y[v]; }
+            } else g.out[0][o] = x[v] + y[v];
         }
     }
 }
@@ -819,8 +867,7 @@ __global__ __launch_bounds__(256) void product_join_kernel(const T* __restrict__
         if constexpr (EPI == GATED) {
             out0[at] = gated_fun(fun, x) * y;
             if (out1) { out1[at] = x; out2[at] = y; }
-        } else if constexpr (EPI == SUM) out0[at] = x + y;
-        else {
+        } else {
             out0[at] = x;
             if (PAIRED) out1[at] = y;
         }
@@ -938,53 +985,49 @@ static void launch_product(Device* dev, Product<T> g, const Split& s, bool a_alo
     hipLaunchKernelGGL((product_join_kernel<T, PAIRED, EPI>), dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, dev->stream, partial, s.parts, n, g.fun, out[0], out[1], out[2]);
 }
 
-// The products of up to 64 rows.  one_a: both products have the same A (GATED), else each has its own (SUM).
-struct FewPlan { int row_tiles, groups, parts, steps_per_part; };
+// The products of up to 64 rows: GATED, where both have the same A, or SUM, where each has its own.
+struct FewPlan { int row_tiles, width, groups, parts, steps_per_part; };
 template <typename T>
-static FewPlan few_plan(const Device* dev, int64_t rows, int64_t cols, int64_t inner) {
+static FewPlan few_plan(const Device* dev, int64_t rows, int64_t cols, int64_t inner, bool along) {
     FewPlan f;
     const int64_t cus = dev->props.multiProcessorCount, chunk = 64 / (int64_t)sizeof(T), chunks = inner / chunk;
     f.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    f.groups = (int)((cols + 15) / 16);
-    // parts of the contraction for columns that fill less than half of the units, 32 chunks per part at least
-    int64_t parts = f.groups * 2 > cus ? 1 : cus / f.groups;
-    if (parts > chunks / 32) parts = chunks / 32 > 0 ? chunks / 32 : 1;
+    f.width = sizeof(T) == 4 && !along && cols > 1 ? 2 : 1;              // 128 bytes of a row of weights
+    f.groups = (int)((cols + 16 * f.width - 1) / (16 * f.width));
+    // one block per unit at least where the contraction is long enough: 16 chunks a part keep all wavefronts busy
+    int64_t parts = f.groups >= cus ? 1 : (cus + f.groups - 1) / f.groups;
+    if (parts > chunks / 16) parts = chunks / 16 > 0 ? chunks / 16 : 1;
     f.steps_per_part = chunks ? (int)((chunks + parts - 1) / parts) : 1;
+    f.steps_per_part += f.steps_per_part & 1;                            // (chunks are taken in twos)
     f.parts = chunks ? (int)((chunks + f.steps_per_part - 1) / f.steps_per_part) : 1;
     return f;
 }
-static uint64_t few_partial_elements(const FewPlan& f, int64_t rows, int64_t cols) { return f.parts > 1 ? (uint64_t)f.parts * 2 * rows * cols : 0; }
+// the parts' sums, in elements: whole fragments of 16 x 16
+static uint64_t few_partial_elements(const FewPlan& f) { return f.parts > 1 ? (uint64_t)f.parts * f.groups * 2 * f.row_tiles * f.width * 256 : 0; }
 
 template <typename T, int EPI>
 static int launch_few(Device* dev, Product<T> g, const FewPlan& f, bool along, T* partial) {
-    constexpr int WAVES = 8;
     g.tiles_n = f.groups; g.steps_per_part = f.steps_per_part;
-    const int64_t n = (int64_t)g.rows * g.cols;
-    T* const out[3] = {g.out[0], g.out[1], g.out[2]};
-    if (f.parts > 1) { g.out[0] = partial; g.out[1] = partial + n; g.out[2] = nullptr; g.part_stride = 2 * n; }
+    unsigned* arrived = nullptr;
+    if (f.parts > 1) {
+        NK_REQUIRE((unsigned)f.groups <= ARRIVALS, "nk_gated_matmul: %d groups of columns share their sums, %u can", f.groups, ARRIVALS);
+        if (int e = arrivals(dev, &arrived)) return e;
+    }
     hipError_t refused = hipSuccess;
-    const auto go = [&](auto rt, auto epi) {
-        constexpr int RT = decltype(rt)::value, E = decltype(epi)::value;
-        const unsigned bytes = WAVES * 2 * RT * 64 * 4 * sizeof(T);
+    const auto go = [&](auto rt) {
+        constexpr int RT = decltype(rt)::value;
+        const unsigned bytes = 8 * 2 * RT * f.width * 64 * 4 * sizeof(T);
         const auto run = [&](auto kernel) {
             if (bytes > 65536) refused = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-            if (refused == hipSuccess) hipLaunchKernelGGL(kernel, dim3((unsigned)(f.groups * f.parts)), dim3(WAVES * 64), bytes, dev->stream, g);
+            if (refused == hipSuccess) hipLaunchKernelGGL(kernel, dim3((unsigned)(f.groups * f.parts)), dim3(512), bytes, dev->stream, g, f.parts, partial, arrived);
         };
-        if (along) run(few_rows_kernel<T, RT, 1, WAVES, true, E>);
-        else       run(few_rows_kernel<T, RT, 1, WAVES, false, E>);
+        if (along) run(few_rows_kernel<T, RT, 1, true, EPI>);
+        else if (f.width == 1) run(few_rows_kernel<T, RT, 1, false, EPI>);
+        else if constexpr (sizeof(T) == 4) run(few_rows_kernel<T, RT, 2, false, EPI>);
     };
-    const auto rows = [&](auto epi) {
-        if (f.row_tiles == 1)      go(std::integral_constant<int, 1>(), epi);
-        else if (f.row_tiles == 2) go(std::integral_constant<int, 2>(), epi);
-        else                       go(std::integral_constant<int, 4>(), epi);
-    };
-    if (f.parts == 1) rows(std::integral_constant<int, EPI>());
-    else {
-        // (with parts the two products of a GATED call still share their A, which STORE does not know: A[1] = A[0])
-        g.A[1] = g.A[1] ? g.A[1] : g.A[0];
-        rows(std::integral_constant<int, STORE>());
-        hipLaunchKernelGGL((product_join_kernel<T, true, EPI>), dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, dev->stream, partial, f.parts, n, g.fun, out[0], out[1], out[2]);
-    }
+    if (f.row_tiles == 1)      go(std::integral_constant<int, 1>());
+    else if (f.row_tiles == 2) go(std::integral_constant<int, 2>());
+    else                       go(std::integral_constant<int, 4>());
     NK_HIP(refused);
     return NK_OK;
 }
@@ -1011,8 +1054,8 @@ static int gated_forward(Device* dev, int fun, bool along, int64_t M, int64_t K,
     g.out[0] = H; g.out[1] = gate; g.out[2] = up;
     void* ws = nullptr;
     if (M <= 64) {
-        const FewPlan f = few_plan<T>(dev, M, N, K);
-        if (const uint64_t need = few_partial_elements(f, M, N))
+        const FewPlan f = few_plan<T>(dev, M, N, K, along);
+        if (const uint64_t need = few_partial_elements(f))
             if (int e = workspace(dev, need * sizeof(T), &ws)) return e;
         if (int e = launch_few<T, GATED>(dev, g, f, along, (T*)ws)) return e;
         NK_HIP(hipGetLastError());
@@ -1043,13 +1086,14 @@ static int gated_backward(Device* dev, int fun, bool along, int64_t M, int64_t K
                           const T* E, T* dX, T* dWg, T* dWu) {
     const int64_t n = M * N;
     const Split sx = plan<T>(dev, false, M, K, N, 2), sw = plan<T>(dev, true, K, N, M, 1);
-    const FewPlan few = few_plan<T>(dev, M, K, N);
-    const uint64_t px = dX ? M <= 64 ? few_partial_elements(few, M, K) : partial_elements(sx, false, M, K) : 0, pw = dWg ? partial_elements(sw, true, K, N) : 0;
+    const FewPlan few = few_plan<T>(dev, M, K, N, !along);
+    const uint64_t px = dX ? M <= 64 ? few_partial_elements(few) : partial_elements(sx, false, M, K) : 0, pw = dWg ? partial_elements(sw, true, K, N) : 0;
     const bool two_x = dX && two_planes<T>(M, K, 2 * N), two_w = dWg && two_planes<T>(K, 2 * N, M) && M > 64;
     const uint64_t scales_x = two_x ? M + K : 0, scales_w = two_w ? K + 2 * N : 0;
     void* ws = nullptr;
-    if (int e = workspace(dev, (2 * (uint64_t)n + (px > pw ? px : pw)) * sizeof(T) + (scales_x + scales_w) * sizeof(int), &ws)) return e;
-    T *const dg = (T*)ws, *const du = dg + n, *const partial = du + n;
+    const uint64_t room = (2 * (uint64_t)n + 15) & ~(uint64_t)15;            // both errors; what follows starts at a whole vector
+    if (int e = workspace(dev, (room + (px > pw ? px : pw)) * sizeof(T) + (scales_x + scales_w) * sizeof(int), &ws)) return e;
+    T *const dg = (T*)ws, *const du = dg + n, *const partial = dg + room;
     hipLaunchKernelGGL((gated_errors_kernel<T>), dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, dev->stream, fun, n, E, gate, up, dg, du);
     Product<T> gx{}, gw{};
     gx.A[0] = dg; gx.A[1] = du; gx.lda = N; gx.B[0] = Wg; gx.B[1] = Wu; gx.ldb = along ? K : N;      // (weights stored by row have neighbours along N)

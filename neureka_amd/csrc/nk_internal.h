@@ -39,6 +39,8 @@ struct Device {
     void* workspace = nullptr;
     uint64_t workspace_bytes = 0;
     int big_tiles = 0;                   // matmul's kernels that need more LDS than a launch gets by default: 0 not asked yet, 1 granted, -1 not available
+    // arrival counters of blocks that share one result: zero between launches (the last to arrive sets its counter back)
+    unsigned* arrivals = nullptr;
     // this device's copy of the file-scope array nk_sum_static keeps its partial results in
     void* sum_static_scratch = nullptr;
 };
@@ -47,6 +49,8 @@ int set_error(int code, const char* fmt, ...);
 void set_path(const char* name);
 std::shared_ptr<Device> device_ref(nk_dev h);   // empty (and error set) if unknown; keeps the device alive across a concurrent close
 int workspace(Device* dev, uint64_t bytes, void** out);
+constexpr unsigned ARRIVALS = 1024;
+int arrivals(Device* dev, unsigned** out);   // ARRIVALS counters, allocated with the first call
 int stats_static_init(Device* dev);     // resolves sum_static_scratch; the device must be current
 int memory_release_all(Device* dev);    // nk_device_close: live buffers, blocks at rest and staging chunks go back to the driver
 void launch_fill_bytes(Device* dev, void* dst, uint64_t bytes, uint64_t pattern8);   // 16-byte aligned dst, bytes a multiple of 16

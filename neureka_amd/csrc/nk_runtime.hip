@@ -46,6 +46,18 @@ int workspace(Device* dev, uint64_t bytes, void** out) {
     return NK_OK;
 }
 
+int arrivals(Device* dev, unsigned** out) {
+    if (!dev->arrivals) {
+        void* p = nullptr;
+        NK_HIP(hipMalloc(&p, ARRIVALS * sizeof(unsigned)));
+        launch_fill_bytes(dev, p, ARRIVALS * sizeof(unsigned), 0);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) { (void)hipFree(p); NK_HIP(e); }
+        dev->arrivals = (unsigned*)p;
+    }
+    *out = dev->arrivals;
+    return NK_OK;
+}
+
 int check_cfg(const char* what, const int32_t* cfg, int rank) {
     NK_REQUIRE(cfg != nullptr, "%s: null view descriptor", what);
     NK_REQUIRE(rank >= 1 && rank <= NK_MAX_RANK, "%s: rank %d outside [1, %d]", what, rank, NK_MAX_RANK);
@@ -234,6 +246,8 @@ int nk_device_close(nk_dev h) {
     (void)memory_release_all(dev);
     if (dev->workspace) (void)hipFree(dev->workspace);
     dev->workspace = nullptr; dev->workspace_bytes = 0;
+    if (dev->arrivals) (void)hipFree(dev->arrivals);
+    dev->arrivals = nullptr;
     dev->closed = true;                  // the object itself lives until the last call that holds a reference returns
     NK_HIP(hipStreamDestroy(dev->stream));
     std::lock_guard<std::mutex> lock(g_devices_mu);
