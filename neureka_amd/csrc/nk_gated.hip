@@ -99,13 +99,13 @@ struct Share {
     }
 };
 
-// 128 x 128 tiles, 4 wavefronts of 64 x 64, slices of 16 l in two LDS buffers.  f64: 64 x 64 x 16 multiply-adds are 16 x 4 matrix
-// instructions against 32 LDS reads of 8 bytes a lane.
-template <typename T, bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
+// F x F fragments of 16 x 16 per wavefront, 4 wavefronts: tiles of 128 x 128 (F = 4) or 64 x 64, slices of 16 l in two LDS buffers.  f64,
+// F = 4: 64 x 64 x 16 multiply-adds are 16 x 4 matrix instructions against 32 LDS reads of 8 bytes a lane.
+template <typename T, int F, bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
 __global__ __launch_bounds__(256) void product_kernel(const Product<T> g) {
     typedef Quad<T> Q;
     typedef typename Q::Acc Acc;
-    constexpr int BM = 128, BN = 128, BK = 16;
+    constexpr int BM = 32 * F, BN = 32 * F, BK = 16;
     __shared__ T a_lds[2][BM * BK], b_lds[2][BN * BK];
     const unsigned tiles = (unsigned)(g.tiles_m * g.tiles_n), part = blockIdx.x / tiles;
     int tm, tn;
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(256) void product_kernel(const Product<T> g) {
         a.load(g.A[segment] + am * (A_ALONG ? g.lda : 1), g.lda, l0, g.inner, t);
         b.load(g.B[PAIRED ? half : segment] + bn * (B_ALONG ? g.ldb : 1), g.ldb, l0, g.inner, t);
     };
-    Acc acc[4][4] = {};
+    Acc acc[F][F] = {};
     request(first);
     a.store(a_lds[0], t); b.store(b_lds[0], t);
     if (first + 1 < last) request(first + 1);
@@ -137,18 +137,18 @@ __global__ __launch_bounds__(256) void product_kernel(const Product<T> g) {
         const T *const ap = a_lds[cur] + lane, *const bp = b_lds[cur] + lane;
 #pragma unroll
         for (int k = 0; k < BK / 4; k++) {
-            T af[4], bf[4];
+            T af[F], bf[F];
 #pragma unroll
-            for (int i = 0; i < 4; i++) af[i] = ap[((wm * 4 + i) * (BK / 4) + k) * 64];
+            for (int i = 0; i < F; i++) af[i] = ap[((wm * F + i) * (BK / 4) + k) * 64];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int block = PAIRED ? (j >> 1) * 4 + wn * 2 + (j & 1) : wn * 4 + j;
+            for (int j = 0; j < F; j++) {
+                const int block = PAIRED ? (j / (F / 2)) * F + wn * (F / 2) + j % (F / 2) : wn * F + j;
                 bf[j] = bp[(block * (BK / 4) + k) * 64];
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < F; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = Q::mma(af[i], bf[j], acc[i][j]);
+                for (int j = 0; j < F; j++) acc[i][j] = Q::mma(af[i], bf[j], acc[i][j]);
         }
         if (s + 1 < last) {
             a.store(a_lds[cur ^ 1], t); b.store(b_lds[cur ^ 1], t);
@@ -158,20 +158,20 @@ __global__ __launch_bounds__(256) void product_kernel(const Product<T> g) {
     }
     const int64_t shift = (int64_t)part * g.part_stride;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < F; i++)
 #pragma unroll
         for (int v = 0; v < 4; v++) {
-            const int m = m0 + wm * 64 + i * 16 + Q::row(lane, v);
+            const int m = m0 + wm * (16 * F) + i * 16 + Q::row(lane, v);
             if (m >= g.rows) continue;
             const int64_t row = (int64_t)m * g.cols + shift;
 #pragma unroll
-            for (int j = 0; j < (PAIRED ? 2 : 4); j++) {
-                const int n = n0 + (PAIRED ? wn * 32 : wn * 64) + j * 16 + (lane & 15);
+            for (int j = 0; j < (PAIRED ? F / 2 : F); j++) {
+                const int n = n0 + (PAIRED ? wn * (8 * F) : wn * (16 * F)) + j * 16 + (lane & 15);
                 if (n >= g.cols) continue;
                 const T x = acc[i][j][v];
                 if constexpr (!PAIRED) g.out[0][row + n] = x;
                 else {
-                    const T y = acc[i][2 + (j & 1)][v];
+                    const T y = acc[i][F / 2 + j % (F / 2)][v];
                     if constexpr (EPI == GATED) {
                         g.out[0][row + n] = gated_fun(g.fun, x) * y;
                         if (g.out[1]) { g.out[1][row + n] = x; g.out[2][row + n] = y; }
@@ -922,19 +922,29 @@ __global__ __launch_bounds__(256) void gated_errors_kernel(int fun, int64_t n, c
 }
 
 // ---- plans ---------------------------------------------------------------------------------------------------------------
-struct Split { bool large; int tiles_m, tiles_n, parts, steps_per_part; };
+struct Split { int edge, tiles_m, tiles_n, parts, steps_per_part; };
 template <typename T>
 static Split plan(const Device* dev, bool paired, int64_t rows, int64_t cols, int64_t inner, int segments) {
     Split s;
     const int64_t cus = dev->props.multiProcessorCount, steps = (sizeof(T) == 4 ? inner / 16 : (inner + 15) / 16) * segments;      // (f32: whole slices)
-    const auto tile = [&](int64_t edge) {
+    const auto tiles_of = [&](int64_t edge) {
+        s.edge = (int)edge;
         s.tiles_m = (int)((rows + edge - 1) / edge);
         s.tiles_n = (int)(paired ? (cols + edge / 2 - 1) / (edge / 2) : (cols + edge - 1) / edge);
         return (int64_t)s.tiles_m * s.tiles_n;
     };
-    s.large = sizeof(T) == 4 && tile(256) >= cus;
-    const int64_t tiles = tile(s.large ? 256 : 128), want = (s.large ? 1 : 2) * cus;
-    int64_t parts = tiles >= want ? 1 : want / tiles;
+    int64_t parts = 1;
+    if constexpr (sizeof(T) == 8) {
+        // 128 x 128 tiles where two per unit exist, else 64 x 64, in parts where not even four of those do
+        if (tiles_of(128) < 2 * cus) {
+            const int64_t tiles = tiles_of(64);
+            if (tiles < 2 * cus) parts = 4 * cus / tiles;
+        }
+    } else {
+        const bool large = tiles_of(256) >= cus;
+        const int64_t tiles = tiles_of(large ? 256 : 128), want = (large ? 1 : 2) * cus;
+        if (tiles < want) parts = want / tiles;
+    }
     if (parts > steps / 8) parts = steps / 8 > 0 ? steps / 8 : 1;
     s.steps_per_part = (int)((steps + parts - 1) / parts);
     if (s.steps_per_part < 1) s.steps_per_part = 1;          // (fewer than 16 l)
@@ -955,14 +965,15 @@ static void launch_tiles(Device* dev, const Product<float>& g, const Split& s, d
     };
     const auto go = [&](auto scaled) {
         constexpr bool S = decltype(scaled)::value;
-        if (s.large) run(split_product_kernel<S, 2, 4, 4, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 512, 256);
-        else         run(split_product_kernel<S, 2, 2, 2, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 256, 128);
+        if (s.edge == 256) run(split_product_kernel<S, 2, 4, 4, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 512, 256);
+        else               run(split_product_kernel<S, 2, 2, 2, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 256, 128);
     };
     if (g.a_scale) go(std::true_type()); else go(std::false_type());
 }
 template <bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
-static void launch_tiles(Device* dev, const Product<double>& g, const Split&, dim3 grid) {
-    hipLaunchKernelGGL((product_kernel<double, A_ALONG, B_ALONG, PAIRED, EPI>), grid, dim3(256), 0, dev->stream, g);
+static void launch_tiles(Device* dev, const Product<double>& g, const Split& s, dim3 grid) {
+    if (s.edge == 128) hipLaunchKernelGGL((product_kernel<double, 4, A_ALONG, B_ALONG, PAIRED, EPI>), grid, dim3(256), 0, dev->stream, g);
+    else               hipLaunchKernelGGL((product_kernel<double, 2, A_ALONG, B_ALONG, PAIRED, EPI>), grid, dim3(256), 0, dev->stream, g);
 }
 
 template <typename T, bool PAIRED, int EPI>
