@@ -78,24 +78,43 @@ __device__ __forceinline__ void own_tile(unsigned block, unsigned tiles, int til
     tn = (int)(in / height);
 }
 
-// One operand's share of a slice: `WIDTH` rows of the result (or columns, for B) by 16 steps of l, 256 threads, E consecutive l each.
+__device__ __forceinline__ void lds_barrier() {             // orders LDS only: requests to memory stay in flight
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// One operand's share of a slice: `WIDTH` rows of the result (or columns, for B) by 16 steps of l, 256 threads, E consecutive l
+// each; two slices on their way.
 template <typename T, int WIDTH, bool ALONG>
 struct Share {
-    static constexpr int BK = 16, E = WIDTH * BK / 256, PER_ROW = BK / E;
-    T v[E];
-    // `row`: the operand's first element of this thread's row; `l0`: the slice's first l
+    static constexpr int BK = 16, E = WIDTH * BK / 256, PER_ROW = BK / E, V = 16 / sizeof(T);
+    T v[2][E];
     static __device__ __forceinline__ int row_of(int t) { return ALONG ? t / PER_ROW : t % WIDTH; }
-    static __device__ __forceinline__ int l_of(int t) { return (ALONG ? t % PER_ROW : t / WIDTH) * E; }
+    static __device__ __forceinline__ int l_of(int t) { return ALONG ? (t % PER_ROW) * E : __builtin_amdgcn_readfirstlane(t / WIDTH) * E; }
+    // `row`: the operand's first element of this thread's row; `l0`: the slice's first l.  WHOLE: all 16 l of the slice exist; else what
+    // lies past `inner` is zero.
+    template <int SET, bool WHOLE>
     __device__ __forceinline__ void load(const T* row, int64_t ld, int l0, int inner, int t) {
         const int l = l0 + l_of(t);
+        if constexpr (ALONG && WHOLE) {
+            typedef T Vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
 #pragma unroll
-        for (int e = 0; e < E; e++) v[e] = l + e < inner ? row[(int64_t)(l + e) * (ALONG ? 1 : ld)] : T(0);
+            for (int u = 0; u < E / V; u++) {
+                const Vec x = *(const Vec*)(row + l + u * V);
+#pragma unroll
+                for (int e = 0; e < V; e++) v[SET][u * V + e] = x[e];
+            }
+        } else
+#pragma unroll
+            for (int e = 0; e < E; e++) v[SET][e] = WHOLE || l + e < inner ? row[(int64_t)(l + e) * (ALONG ? 1 : ld)] : T(0);
     }
     // LDS: fragments of 16 rows x 4 l, in the order in which the lanes of a wavefront hold them
+    template <int SET>
     __device__ __forceinline__ void store(T* lds, int t) const {
         const int r = row_of(t), l = l_of(t);
 #pragma unroll
-        for (int e = 0; e < E; e++) lds[((r >> 4) * (BK / 4) + ((l + e) >> 2)) * 64 + ((l + e) & 3) * 16 + (r & 15)] = v[e];
+        for (int e = 0; e < E; e++) lds[((r >> 4) * (BK / 4) + ((l + e) >> 2)) * 64 + ((l + e) & 3) * 16 + (r & 15)] = v[SET][e];
     }
 };
 
@@ -119,22 +138,24 @@ __global__ __launch_bounds__(256) void product_kernel(const Product<T> g) {
     const int64_t am = m0 + a.row_of(t) < g.rows ? m0 + a.row_of(t) : g.rows - 1;
     const int bt = b.row_of(t), half = PAIRED ? bt / HALF : 0, bc = n0 + (PAIRED ? bt % HALF : bt);
     const int64_t bn = bc < g.cols ? bc : g.cols - 1;
-    const int per_segment = (g.inner + BK - 1) / BK;
-    const int first = (int)part * g.steps_per_part, all = per_segment * g.segments;
+    // whole slices of all segments first, g.steps_per_part of them per part; the last part also takes what is left of each segment
+    const int whole = g.inner / BK, all = whole * g.segments;
+    const int first = (int)part * g.steps_per_part < all ? (int)part * g.steps_per_part : all;
     const int last = first + g.steps_per_part < all ? first + g.steps_per_part : all;
-    const auto request = [&](int s) {
-        const int segment = s / per_segment, l0 = (s - segment * per_segment) * BK;
-        a.load(g.A[segment] + am * (A_ALONG ? g.lda : 1), g.lda, l0, g.inner, t);
-        b.load(g.B[PAIRED ? half : segment] + bn * (B_ALONG ? g.ldb : 1), g.ldb, l0, g.inner, t);
+    const auto request = [&](auto set, auto complete, int segment, int l0) {
+        constexpr int SET = decltype(set)::value;
+        constexpr bool WHOLE = decltype(complete)::value;
+        a.template load<SET, WHOLE>(g.A[segment] + am * (A_ALONG ? g.lda : 1), g.lda, l0, g.inner, t);
+        b.template load<SET, WHOLE>(g.B[PAIRED ? half : segment] + bn * (B_ALONG ? g.ldb : 1), g.ldb, l0, g.inner, t);
+    };
+    const auto request_slice = [&](auto set, int s) {        // past the end: the last one once more
+        s = s < last ? s : last - 1;
+        const int segment = s >= whole;
+        request(set, std::true_type(), segment, (s - segment * whole) * BK);
     };
     Acc acc[F][F] = {};
-    request(first);
-    a.store(a_lds[0], t); b.store(b_lds[0], t);
-    if (first + 1 < last) request(first + 1);
-    __syncthreads();
-    for (int s = first; s < last; s++) {
-        const int cur = (s - first) & 1;
-        const T *const ap = a_lds[cur] + lane, *const bp = b_lds[cur] + lane;
+    const auto multiply = [&](int buffer) {
+        const T *const ap = a_lds[buffer] + lane, *const bp = b_lds[buffer] + lane;
 #pragma unroll
         for (int k = 0; k < BK / 4; k++) {
             T af[F], bf[F];
@@ -150,12 +171,35 @@ __global__ __launch_bounds__(256) void product_kernel(const Product<T> g) {
 #pragma unroll
                 for (int j = 0; j < F; j++) acc[i][j] = Q::mma(af[i], bf[j], acc[i][j]);
         }
-        if (s + 1 < last) {
-            a.store(a_lds[cur ^ 1], t); b.store(b_lds[cur ^ 1], t);
-            if (s + 2 < last) request(s + 2);
-        }
-        __syncthreads();
+    };
+    typedef std::integral_constant<int, 0> Even;
+    typedef std::integral_constant<int, 1> Odd;
+    if (first < last) {
+        // slice s is in LDS, s + 1 and s + 2 in registers or on their way
+        request_slice(Even(), first);
+        request_slice(Odd(), first + 1);
+        a.template store<0>(a_lds[0], t); b.template store<0>(b_lds[0], t);
+        request_slice(Even(), first + 2);
+        lds_barrier();
+        const auto slice = [&](auto parity, int s) {
+            constexpr int P = decltype(parity)::value;
+            a.template store<1 - P>(a_lds[1 - P], t); b.template store<1 - P>(b_lds[1 - P], t);
+            request_slice(std::integral_constant<int, 1 - P>(), s + 3);
+            multiply(P);
+            lds_barrier();
+        };
+        int s = first;
+        for (; s + 1 < last; s += 2) { slice(Even(), s); slice(Odd(), s + 1); }
+        if (s < last) slice(Even(), s);
     }
+    if (g.inner % BK != 0 && last == all)
+        for (int segment = 0; segment < g.segments; segment++) {
+            request(Even(), std::false_type(), segment, whole * BK);
+            a.template store<0>(a_lds[0], t); b.template store<0>(b_lds[0], t);
+            lds_barrier();
+            multiply(0);
+            lds_barrier();
+        }
     const int64_t shift = (int64_t)part * g.part_stride;
 #pragma unroll
     for (int i = 0; i < F; i++)
@@ -412,12 +456,6 @@ struct SplitShare {
         }
     }
 };
-
-__device__ __forceinline__ void lds_barrier() {             // orders LDS only: requests to memory stay in flight
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
 
 // WM x WN wavefronts, each with a tile of FI x FJ fragments of 32 x 32.  PAIRED: the first half of a wavefront's column
 // fragments comes from the first product, the second half from the second.
@@ -926,7 +964,7 @@ struct Split { int edge, tiles_m, tiles_n, parts, steps_per_part; };
 template <typename T>
 static Split plan(const Device* dev, bool paired, int64_t rows, int64_t cols, int64_t inner, int segments) {
     Split s;
-    const int64_t cus = dev->props.multiProcessorCount, steps = (sizeof(T) == 4 ? inner / 16 : (inner + 15) / 16) * segments;      // (f32: whole slices)
+    const int64_t cus = dev->props.multiProcessorCount, steps = inner / 16 * segments;      // whole slices
     const auto tiles_of = [&](int64_t edge) {
         s.edge = (int)edge;
         s.tiles_m = (int)((rows + edge - 1) / edge);
