@@ -286,11 +286,11 @@ template <> struct Partial<2> {
     }
 };
 
-// The exponents of up to three operands' rows (`count` rows of `length`, together with those of a second matrix where there is
+// The exponents of up to five operands' rows (`count` rows of `length`, together with those of a second matrix where there is
 // one), blocks dealt out operand by operand.  Rows that lie along memory: a wavefront each, 64 stretches of every 64th 4
 // elements.  Rows across memory: 32 of them per block, 64 stretches of every 64th element.  Read once at memory speed.
 struct ScaleJob { const float* p[2]; int64_t ld; int count, length; bool along; int* out; unsigned blocks; };
-struct ScaleJobs { ScaleJob job[3]; int n; };
+struct ScaleJobs { ScaleJob job[5]; int n; };
 __device__ __forceinline__ unsigned magnitude(float x) { return __builtin_bit_cast(unsigned, x) & 0x7fffffffu; }
 __device__ __forceinline__ int exponent_for(unsigned largest, int low, int some) {      // low of some non-zero stretches are far below the largest
     if (largest >= 0x7f800000u || 4 * low > some) return MARKED;
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(512) void operand_scales_kernel(const ScaleJobs job
         if (!j.p[k]) continue;
         if (c + 4 <= j.count) {
             const float* const at = j.p[k] + c;
-#pragma unroll 4
+#pragma unroll 8
             for (int l = first; l < j.length; l += 64) {
                 const f32x4 v = *(const f32x4_any*)(at + (int64_t)l * j.ld);
 #pragma unroll
@@ -960,35 +960,36 @@ __global__ __launch_bounds__(256) void gated_errors_kernel(int fun, int64_t n, c
 }
 
 // ---- plans ---------------------------------------------------------------------------------------------------------------
-struct Split { int edge, tiles_m, tiles_n, parts, steps_per_part; };
+struct Split { int edge_m, edge_n, tiles_m, tiles_n, parts, steps_per_part; };
+// What a slice of 16 l takes in the kernels of one tile size, in microseconds, and the blocks of it that a unit runs at a time (two planes;
+// with three every entry is near twice as long, which changes no choice): from 2048 x 1024 x 4096 and 4096^3, whole rounds.
+struct TileCost { int edge_m, edge_n, per_unit; double slice_us; };
+template <typename T> constexpr TileCost TILE_COSTS[] = {{256, 256, 1, 1.6}, {256, 128, 1, 0.92}, {128, 128, 2, 1.05}};
+template <> constexpr TileCost TILE_COSTS<double>[] = {{128, 128, 1, 3.0}, {64, 64, 3, 2.4}};
+
+// The tile size and the number of parts of the contraction with the shortest estimate: rounds of blocks times slices, plus, with parts, a
+// launch that reads them all and writes the sum.
 template <typename T>
 static Split plan(const Device* dev, bool paired, int64_t rows, int64_t cols, int64_t inner, int segments) {
-    Split s;
     const int64_t cus = dev->props.multiProcessorCount, steps = inner / 16 * segments;      // whole slices
-    const auto tiles_of = [&](int64_t edge) {
-        s.edge = (int)edge;
-        s.tiles_m = (int)((rows + edge - 1) / edge);
-        s.tiles_n = (int)(paired ? (cols + edge / 2 - 1) / (edge / 2) : (cols + edge - 1) / edge);
-        return (int64_t)s.tiles_m * s.tiles_n;
-    };
-    int64_t parts = 1;
-    if constexpr (sizeof(T) == 8) {
-        // 128 x 128 tiles where two per unit exist, else 64 x 64, in parts where not even four of those do
-        if (tiles_of(128) < 2 * cus) {
-            const int64_t tiles = tiles_of(64);
-            if (tiles < 2 * cus) parts = 4 * cus / tiles;
+    Split best{};
+    double best_us = 0;
+    for (const TileCost& c : TILE_COSTS<T>) {
+        Split s{};
+        s.edge_m = c.edge_m; s.edge_n = c.edge_n;
+        s.tiles_m = (int)((rows + c.edge_m - 1) / c.edge_m);
+        s.tiles_n = (int)(paired ? (cols + c.edge_n / 2 - 1) / (c.edge_n / 2) : (cols + c.edge_n - 1) / c.edge_n);
+        const int64_t tiles = (int64_t)s.tiles_m * s.tiles_n, slots = c.per_unit * cus;
+        for (int64_t parts = 1; parts <= 16 && (parts == 1 || (steps / parts >= 8 && tiles * parts < 2 * slots + tiles)); parts++) {
+            s.steps_per_part = steps > 0 ? (int)((steps + parts - 1) / parts) : 1;
+            s.parts = steps > 0 ? (int)((steps + s.steps_per_part - 1) / s.steps_per_part) : 1;
+            const double rounds = (double)((tiles * s.parts + slots - 1) / slots);
+            double us = rounds * (s.steps_per_part * c.slice_us + 4.0);
+            if (s.parts > 1) us += 4.0 + (2.0 * s.parts + 1) * (paired ? 2 : 1) * rows * cols * sizeof(T) / 4.5e6;
+            if (best.parts == 0 || us < best_us) { best = s; best_us = us; }
         }
-    } else {
-        const bool large = tiles_of(256) >= cus;
-        const int64_t tiles = tiles_of(large ? 256 : 128), want = (large ? 1 : 2) * cus;
-        if (tiles < want) parts = want / tiles;
     }
-    if (parts > steps / 8) parts = steps / 8 > 0 ? steps / 8 : 1;
-    s.steps_per_part = (int)((steps + parts - 1) / parts);
-    if (s.steps_per_part < 1) s.steps_per_part = 1;          // (fewer than 16 l)
-    s.parts = (int)((steps + s.steps_per_part - 1) / s.steps_per_part);
-    if (s.parts < 1) s.parts = 1;
-    return s;
+    return best;
 }
 static uint64_t partial_elements(const Split& s, bool paired, int64_t rows, int64_t cols) {
     return s.parts > 1 ? (uint64_t)s.parts * (paired ? 2 : 1) * rows * cols : 0;
@@ -996,21 +997,22 @@ static uint64_t partial_elements(const Split& s, bool paired, int64_t rows, int6
 
 template <bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
 static void launch_tiles(Device* dev, const Product<float>& g, const Split& s, dim3 grid) {
-    const auto run = [&](auto kernel, int threads, unsigned edge) {
-        const unsigned lds = 2 * 3 * 2 * edge * 32;          // two buffers of three planes of both operands
+    const auto run = [&](auto kernel, int threads) {
+        const unsigned lds = 2 * 3 * (s.edge_m + s.edge_n) * 32;          // two buffers of three planes of both operands
         (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, dev->stream, g);
     };
     const auto go = [&](auto scaled) {
         constexpr bool S = decltype(scaled)::value;
-        if (s.edge == 256) run(split_product_kernel<S, 2, 4, 4, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 512, 256);
-        else               run(split_product_kernel<S, 2, 2, 2, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 256, 128);
+        if (s.edge_n == 256)      run(split_product_kernel<S, 2, 4, 4, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 512);
+        else if (s.edge_m == 256) run(split_product_kernel<S, 4, 2, 2, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 512);
+        else                      run(split_product_kernel<S, 2, 2, 2, 2, A_ALONG, B_ALONG, PAIRED, EPI>, 256);
     };
     if (g.a_scale) go(std::true_type()); else go(std::false_type());
 }
 template <bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
 static void launch_tiles(Device* dev, const Product<double>& g, const Split& s, dim3 grid) {
-    if (s.edge == 128) hipLaunchKernelGGL((product_kernel<double, 4, A_ALONG, B_ALONG, PAIRED, EPI>), grid, dim3(256), 0, dev->stream, g);
+    if (s.edge_m == 128) hipLaunchKernelGGL((product_kernel<double, 4, A_ALONG, B_ALONG, PAIRED, EPI>), grid, dim3(256), 0, dev->stream, g);
     else               hipLaunchKernelGGL((product_kernel<double, 2, A_ALONG, B_ALONG, PAIRED, EPI>), grid, dim3(256), 0, dev->stream, g);
 }
 
@@ -1152,23 +1154,20 @@ static int gated_backward(Device* dev, int fun, bool along, int64_t M, int64_t K
     gw.rows = (int)K; gw.cols = (int)N; gw.inner = (int)M; gw.segments = 1;
     gw.out[0] = dWg; gw.out[1] = dWu;
     if constexpr (sizeof(T) == 4) {
-        int* const scales = (int*)(partial + (px > pw ? px : pw));
+        int *const scales = (int*)(partial + (px > pw ? px : pw)), *const at = scales + scales_x;
+        ScaleJobs jobs{};
         if (two_x) {
-            ScaleJobs jobs{};
             add_job(jobs, dg, du, N, M, N, true, scales);
             add_job(jobs, Wg, Wu, gx.ldb, K, N, !along, scales + M);
-            launch_scales(dev, jobs);
             gx.a_scale = scales; gx.b_scale[0] = scales + M;
         }
         if (two_w) {
-            int* const at = scales + scales_x;
-            ScaleJobs jobs{};
             add_job(jobs, X, nullptr, K, K, M, false, at);
             add_job(jobs, dg, nullptr, N, N, M, false, at + K);
             add_job(jobs, du, nullptr, N, N, M, false, at + K + N);
-            launch_scales(dev, jobs);
             gw.a_scale = at; gw.b_scale[0] = at + K; gw.b_scale[1] = at + K + N;
         }
+        if (jobs.n) launch_scales(dev, jobs);
     }
     if (dX) {
         if (M <= 64) { if (int e = launch_few<T, SUM>(dev, gx, few, !along, partial)) return e; }
