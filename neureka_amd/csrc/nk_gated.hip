@@ -241,7 +241,6 @@ __global__ __launch_bounds__(256) void product_kernel(const Product<T> g) {
 // 2^15; what is 2^-16 of that or more keeps all its bits, and smaller numbers are off by at most 2^-40 of the largest.
 // A row where that could show -- more than a quarter of its 64 stretches hold nothing beyond 2^-16 of the largest (and are not all
 // zero), or an infinity or NaN -- is marked, and tiles with a marked row take three planes.
-constexpr int64_t TWO_PLANES_FROM = (int64_t)1 << 32;        // multiply-adds
 constexpr int MARKED = 1 << 30;                              // in place of a row's exponent
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -732,7 +731,7 @@ template <typename T, int RT, int CW, bool ALONG, int EPI>
 __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int parts, T* partial, unsigned* arrived) {
     typedef Quad<T> Q;
     typedef typename Q::Acc Acc;
-    constexpr int WAVES = 8, V = 16 / sizeof(T), KC = 4 * V, U = RT > 2 && !ALONG ? 1 : 2, NA = EPI == GATED ? 1 : 2, FRAGMENTS = RT * CW;
+    constexpr int WAVES = 8, V = 16 / sizeof(T), KC = 4 * V, U = 2, NA = EPI == GATED ? 1 : 2, FRAGMENTS = RT * CW;
     typedef T VecV __attribute__((ext_vector_type(V), aligned(sizeof(T))));
     typedef T VecC __attribute__((ext_vector_type(CW), aligned(sizeof(T))));
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
@@ -1083,10 +1082,18 @@ static int launch_few(Device* dev, Product<T> g, const FewPlan& f, bool along, T
     return NK_OK;
 }
 
-// Whether a product of that many multiply-adds takes two planes: they save half of its matrix instructions and cost two launches and
-// a read of the operands before it.
+// Whether a product takes two planes.  They save three of six partial products (at 1.1e15 operations a second) and cost a launch that reads
+// both operands.  Forward in microseconds, two planes against three: 512 x 1024 x 1024 29.6 / 29.2, 1024^3 37 / 40,
+// 1111 x 1000 x 2500 68 / 100, 2048^3 144 / 222; 65 x 4096 x 4096, all weights, 74 / 64.
 template <typename T> static bool two_planes(int64_t rows, int64_t cols, int64_t inner) {
-    return sizeof(T) == 4 && rows > 64 && rows * cols * inner >= TWO_PLANES_FROM;
+    const double saved_us = 6.0 * rows * cols * inner / 1.1e9, cost_us = 6.0 + 4.0 * (rows + cols) * inner / 4.5e6;
+    return sizeof(T) == 4 && saved_us > cost_us;
+}
+// Whether M rows go to few_rows_kernel.  Above 32 rows it holds four row tiles per wavefront and is bound by the matrix instructions: in
+// f32, whose tiles run on the faster 16-bit ones, only while the weights are few (64 rows forward, microseconds, few rows / tiles:
+// 1024 x 1024 17 / 20, 300 x 2000 13 / 20, 4096 x 4096 83 / 63; f64 18 / 24, 14 / 17, 109 / 188).
+template <typename T> static bool takes_few_rows(int64_t M, int64_t K, int64_t N) {
+    return M <= 32 || (M <= 64 && (sizeof(T) == 8 || 2 * K * N * (int64_t)sizeof(T) < 48000000));
 }
 static void add_job(ScaleJobs& jobs, const float* p, const float* second, int64_t ld, int64_t count, int64_t length, bool along, int* out) {
     jobs.job[jobs.n++] = {{p, second}, ld, (int)count, (int)length, along, out, (unsigned)(along ? (count + 7) / 8 : (count + 31) / 32)};
@@ -1104,7 +1111,7 @@ static int gated_forward(Device* dev, int fun, bool along, int64_t M, int64_t K,
     g.rows = (int)M; g.cols = (int)N; g.inner = (int)K; g.segments = 1; g.fun = fun;
     g.out[0] = H; g.out[1] = gate; g.out[2] = up;
     void* ws = nullptr;
-    if (M <= 64) {
+    if (takes_few_rows<T>(M, K, N)) {
         const FewPlan f = few_plan<T>(dev, M, N, K, along);
         if (const uint64_t need = few_partial_elements(f))
             if (int e = workspace(dev, need * sizeof(T), &ws)) return e;
@@ -1138,8 +1145,9 @@ static int gated_backward(Device* dev, int fun, bool along, int64_t M, int64_t K
     const int64_t n = M * N;
     const Split sx = plan<T>(dev, false, M, K, N, 2), sw = plan<T>(dev, true, K, N, M, 1);
     const FewPlan few = few_plan<T>(dev, M, K, N, !along);
-    const uint64_t px = dX ? M <= 64 ? few_partial_elements(few) : partial_elements(sx, false, M, K) : 0, pw = dWg ? partial_elements(sw, true, K, N) : 0;
-    const bool two_x = dX && two_planes<T>(M, K, 2 * N), two_w = dWg && two_planes<T>(K, 2 * N, M) && M > 64;
+    const bool is_few = takes_few_rows<T>(M, K, N);
+    const uint64_t px = dX ? is_few ? few_partial_elements(few) : partial_elements(sx, false, M, K) : 0, pw = dWg ? partial_elements(sw, true, K, N) : 0;
+    const bool two_x = dX && !is_few && two_planes<T>(M, K, 2 * N), two_w = dWg && two_planes<T>(K, 2 * N, M);
     const uint64_t scales_x = two_x ? M + K : 0, scales_w = two_w ? K + 2 * N : 0;
     void* ws = nullptr;
     const uint64_t room = (2 * (uint64_t)n + 15) & ~(uint64_t)15;            // both errors; what follows starts at a whole vector
@@ -1170,7 +1178,7 @@ static int gated_backward(Device* dev, int fun, bool along, int64_t M, int64_t K
         if (jobs.n) launch_scales(dev, jobs);
     }
     if (dX) {
-        if (M <= 64) { if (int e = launch_few<T, SUM>(dev, gx, few, !along, partial)) return e; }
+        if (is_few) { if (int e = launch_few<T, SUM>(dev, gx, few, !along, partial)) return e; }
         else launch_product<T, false, STORE>(dev, gx, sx, true, !along, partial);
     }
     if (dWg) launch_product<T, true, STORE>(dev, gw, sw, false, false, partial);
@@ -1184,9 +1192,9 @@ static int check_gated(const char* what, int fun, int dtype, int layout, int64_t
     NK_REQUIRE(fun == NK_FUN_IDY || fun == NK_FUN_RELU || fun == NK_FUN_SIG || fun == NK_FUN_SILU || fun == NK_FUN_GELU || fun == NK_FUN_TANH,
                "%s: function id %d is none of idy, relu, sig, silu, gelu, tanh", what, fun);
     NK_REQUIRE(layout == NK_LAYOUT_ROW_MAJOR || layout == NK_LAYOUT_COLUMN_MAJOR, "%s: unknown layout %d", what, layout);
-    const int64_t most = (int64_t)1 << 31;
+    const int64_t most = (int64_t)1 << 31, longest = most - 1024;       // (a tile past the end of an axis still counts in 32 bits)
     NK_REQUIRE(M >= 1 && K >= 1 && N >= 1, "%s: M, K, N must be positive (got %lld, %lld, %lld)", what, (long long)M, (long long)K, (long long)N);
-    NK_REQUIRE(M < most && K < most && N < most && M * K < most && K * N < most && M * N < most, "%s: operands are limited to 2^31-1 elements", what);
+    NK_REQUIRE(M <= longest && K <= longest && N <= longest && M * K < most && K * N < most && M * N < most, "%s: operands are limited to 2^31-1 elements and axes to 2^31-1024", what);
     return NK_OK;
 }
 struct Piece { const char* name; nk_buf at; uint64_t bytes; };
