@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256) void product_kernel(const Product<T> g) {
 // 3: bfloat16, any operands.  A float is the sum of three, each the rest of the ones before rounded to nearest: 3 x 8 bits hold its 24
 // (below 2^-110 the last leaves bfloat16's range: off by at most 2^-134).  The six largest of the nine partial products are added,
 // x0 y0, x0 y1, x1 y0, x1 y1, x0 y2, x2 y0; the rest is at most 2^-26 of x y each.  A non-finite operand has no such sum
-// (infinity - infinity), so a wavefront that finds a non-finite result computes its tile once more with the f32
+// (infinity - infinity), so a wavefront that finds a non-finite result computes that fragment of its tile once more with the f32
 // instruction, straight from memory: what comes out is what f32 arithmetic gives.
 //
 // 2: half precision, half as many partial products: x0 y0, x0 y1, x1 y0.  Two halves hold a float to 2^-23 of it (2^-25 on average)
@@ -600,18 +600,10 @@ __device__ __forceinline__ void split_product_tile(const Product<float>& g, unsi
 
     // (two planes: the slices' memory takes the exponents of the tile's rows and columns; every row in it is finite, and so is every sum)
     int* const exponents = (int*)lds;
-    bool odd = false;
     if constexpr (PLANES == 2) {
         for (int r = t; r < BM; r += THREADS) exponents[r] = row_exponent(r);
         for (int c = t; c < BN; c += THREADS) exponents[BM + c] = column_exponent(c);
         lds_barrier();
-    } else {
-#pragma unroll
-        for (int i = 0; i < FI; i++)
-#pragma unroll
-            for (int j = 0; j < FJ; j++)
-#pragma unroll
-                for (int v = 0; v < 16; v++) odd |= !(__builtin_fabsf(acc[i][j][v]) < INFINITY);
     }
     // one fragment of the result (PAIRED: the same fragment of both products) to where it belongs.
     // Register v of lane l: row 8 (v / 4) + 4 (l / 32) + v % 4, column l % 32 of the fragment.
@@ -636,22 +628,30 @@ __device__ __forceinline__ void split_product_tile(const Product<float>& g, unsi
         }
     };
     constexpr int SHOWN = PAIRED ? FJ / 2 : FJ;             // fragments per row of the wavefront's tile, of one product
-    if (PLANES == 2 || !__any(odd)) {
+    unsigned again = 0;                                     // fragments with a result that is not finite
 #pragma unroll
-        for (int i = 0; i < FI; i++)
+    for (int i = 0; i < FI; i++)
 #pragma unroll
-            for (int j = 0; j < SHOWN; j++) write(i, j, acc[i][j], acc[i][PAIRED ? FJ / 2 + j : j]);
-        return;
-    }
+        for (int j = 0; j < SHOWN; j++) {
+            const f32x16 &x = acc[i][j], &y = acc[i][PAIRED ? FJ / 2 + j : j];
+            if constexpr (PLANES == 3) {
+                bool odd = false;
+#pragma unroll
+                for (int v = 0; v < 16; v++) odd |= !(__builtin_fabsf(x[v]) < INFINITY) || !(__builtin_fabsf(y[v]) < INFINITY);
+                if (__any(odd)) { again |= 1u << (i * SHOWN + j); continue; }
+            }
+            write(i, j, x, y);
+        }
     if constexpr (PLANES == 3)
 #pragma unroll 1
     for (int f = 0; f < FI * SHOWN; f++) {
+        if (!(again >> f & 1)) continue;
         const int i = f / SHOWN, j = f % SHOWN;
         const int m = m0 + (wm * FI + i) * 32 + (lane & 31), n = n0 + (PAIRED ? wn * (FJ / 2) + j : wn * FJ + j) * 32 + (lane & 31);
         const int64_t am = (int64_t)(m < g.rows ? m : g.rows - 1) * (A_ALONG ? g.lda : 1), bn = (int64_t)(n < g.cols ? n : g.cols - 1) * (B_ALONG ? g.ldb : 1);
         f32x16 x = {}, y = {};
         const int turns = last - first + (last == all && g.inner % 16 != 0 ? g.segments : 0);
-#pragma unroll 1
+#pragma unroll 2
         for (int turn = 0; turn < turns; turn++) {
             const int s = first + turn, left = s - all;
             const int segment = left >= 0 ? left : s >= whole, l0 = (left >= 0 ? whole : s - segment * whole) * 16;
