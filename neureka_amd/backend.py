@@ -418,8 +418,7 @@ class LayerNormAlgorithm(Algorithm):
             raise IllegalArgumentException(f"the epsilon of layerNorm is finite and not negative, not {call.args['epsilon']}")
         src = as_rows(src)
         if call.args["keep"]:
-            rows = src.ndc.size // cols
-            call.args["mean"], call.args["rstd"] = call.device.allocate(src.dtype, rows), call.device.allocate(src.dtype, rows)
+            call.args["stats"] = call.device.allocate(src.dtype, 2 * (src.ndc.size // cols))
         call.inputs = [_new_output(call.device, src.dtype, src.ndc.shape, overwritten=True), src, as_dense(gain), as_dense(bias)]
         return call
 
@@ -747,7 +746,7 @@ def hip_dot(call: ExecutionCall):
 
 def hip_layer_norm(call: ExecutionCall):
     a = call.args
-    call.device.launch_layer_norm(call.input(0), call.input(1), call.input(2), call.input(3), a["epsilon"], a.get("mean"), a.get("rstd"))
+    call.device.launch_layer_norm(call.input(0), call.input(1), call.input(2), call.input(3), a["epsilon"], a.get("stats"))
     return call.input(0)
 
 

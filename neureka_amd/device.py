@@ -70,7 +70,9 @@ class HipData:
             self._freed = True
             self.device._data_objects -= 1
             if not self.device._disposed:
-                _lib.check(self.device._lib.nk_free(self.device.handle, self.ptr))
+                status = self.device._lib.nk_free(self.device.handle, self.ptr)
+                if status:
+                    _lib.check(status)
 
     def __del__(self):  # the role of CustomDeviceCleaner (devices/CustomDeviceCleaner.java:21-121)
         try:
@@ -250,13 +252,14 @@ class HipDevice:
     # ---- data access: AbstractDevice._readAll/_readItem/_readArray/_writeItem/_writeArray ------------
     def allocate(self, dtype, size: int) -> HipData:
         """Device.allocate (OpenCLDevice.java:520-530)."""
-        self._check_open()
-        itemsize = _ITEM_SIZES.get(dtype)
-        if itemsize is None:
-            itemsize = np.dtype(dtype).itemsize
-        ptr = C.c_uint64(0)
-        _lib.check(self._lib.nk_alloc(self.handle, int(size) * itemsize, C.byref(ptr)))
-        return HipData(self, ptr.value, dtype, int(size))
+        if self._disposed:
+            self._check_open()
+        size = int(size)
+        ptr = C.c_uint64()
+        status = self._lib.nk_alloc(self.handle, size * (_ITEM_SIZES.get(dtype) or np.dtype(dtype).itemsize), C.byref(ptr))
+        if status:
+            _lib.check(status)
+        return HipData(self, ptr.value, dtype, size)
 
     def allocateFromOne(self, dtype, size: int, value) -> HipData:
         """Device.allocateFromOne: a buffer filled with one value by the device (OpenCLDevice.java:478-486)."""
@@ -470,29 +473,29 @@ class HipDevice:
             raise IllegalArgumentException(f"the last axis of {what} has to be contiguous and its rows one pitch apart")
         return (t._data.ptr + rows[0] * t.dtype.itemsize,) + rows[1:]
 
-    def launch_layer_norm(self, drn, src, gain, bias, epsilon: float = 1e-5, mean=None, rstd=None) -> None:
-        """drn = (src - mean) * rstd * gain + bias over the last axis; `mean` and `rstd` (one element per row) are written where
-        given.  `drn` may be `src`."""
+    def launch_layer_norm(self, drn, src, gain, bias, epsilon: float = 1e-5, stats=None) -> None:
+        """drn = (src - mean) * rstd * gain + bias over the last axis.  ``stats``, where given, receives what the backward pass
+        needs: the means of all rows, then their reciprocal deviations.  ``drn`` may be ``src``."""
         dt = drn.dtype
         code = _dtype_code(dt)
         at, rows, cols, pitch = self._rows_at("the source", src)
-        if src.dtype != dt or src.shape != drn.shape:
+        if src.dtype != dt or src.ndc.shape != drn.ndc.shape:
             raise IllegalArgumentException(f"source {src.dtype}{list(src.shape)} and drain {dt}{list(drn.shape)} differ")
+        mean = 0 if stats is None else self._dense_at("stats", stats, dt, 2 * rows)
         _lib.check(self._lib.nk_layer_norm(
             self.handle, code, rows, cols, at, pitch, self._dense_at("the gain", gain, dt, cols), self._dense_at("the bias", bias, dt, cols),
-            epsilon, self._dense_at("the drain", drn, dt, rows * cols), 0 if mean is None else self._dense_at("mean", mean, dt, rows),
-            0 if rstd is None else self._dense_at("rstd", rstd, dt, rows)))
+            epsilon, self._dense_at("the drain", drn, dt, rows * cols), mean, mean and mean + rows * dt.itemsize))
 
-    def launch_layer_norm_backward(self, src, gain, mean, rstd, error, d_src=None, d_gain=None, d_bias=None) -> None:
+    def launch_layer_norm_backward(self, src, gain, stats, error, d_src=None, d_gain=None, d_bias=None) -> None:
         """The gradients of launch_layer_norm that are asked for, given the error of its drain."""
         dt = src.dtype
         code = _dtype_code(dt)
         at, rows, cols, pitch = self._rows_at("the source", src)
-        outs = [0 if t is None else self._dense_at(what, t, dt, size) for what, t, size in
-                (("d_src", d_src, rows * cols), ("d_gain", d_gain, cols), ("d_bias", d_bias, cols))]
+        mean = self._dense_at("stats", stats, dt, 2 * rows)
         _lib.check(self._lib.nk_layer_norm_backward(
-            self.handle, code, rows, cols, at, pitch, self._dense_at("the gain", gain, dt, cols), self._dense_at("mean", mean, dt, rows),
-            self._dense_at("rstd", rstd, dt, rows), self._dense_at("the error", error, dt, rows * cols), *outs))
+            self.handle, code, rows, cols, at, pitch, self._dense_at("the gain", gain, dt, cols), mean, mean + rows * dt.itemsize,
+            self._dense_at("the error", error, dt, rows * cols), 0 if d_src is None else self._dense_at("d_src", d_src, dt, rows * cols),
+            0 if d_gain is None else self._dense_at("d_gain", d_gain, dt, cols), 0 if d_bias is None else self._dense_at("d_bias", d_bias, dt, cols)))
 
     def launch_dropout(self, drn, src, probability: float, seed: int, offset: int = 0) -> None:
         """drn = keep ? src / (1 - probability) : 0, keep from (seed, offset) and the element's row-major index."""

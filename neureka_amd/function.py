@@ -112,7 +112,7 @@ def _joint_gradients(call: ExecutionCall, parents: Sequence[Tensor], wanted: Lis
         if op_id == "dropout":                    # the same mask on the error
             device.launch_dropout(out[0], error, args["probability"], args["seed"], args["offset"])
         elif op_id == "layerNorm":
-            device.launch_layer_norm_backward(operands[0], operands[1], args["mean"], args["rstd"], as_dense(error), *out)
+            device.launch_layer_norm_backward(operands[0], operands[1], args["stats"], as_dense(error), *out)
         else:
             d_x, d_gate, d_up = out
             if (d_gate is None) != (d_up is None):               # the kernel computes both

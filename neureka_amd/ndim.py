@@ -99,6 +99,8 @@ class NDConfiguration:
         tensor of a shape and layout."""
         if type(shape) is not tuple:
             shape = tuple(int(s) for s in shape)
+        if layout is Layout.ROW_MAJOR:
+            return _row_major_configuration(shape)
         return _dense_configuration(shape, layout)
 
     @staticmethod
@@ -293,3 +295,9 @@ def _dense_configuration(shape: Tuple[int, ...], layout: Layout) -> NDConfigurat
     # the flat->nd table is always the row-major one for RM and CM tensors (NDConfiguration.getLayout :157-173)
     imap = Layout.ROW_MAJOR.newStridesFor(shape)
     return NDConfiguration.of(shape, strides, imap, (1,) * len(shape), (0,) * len(shape))
+
+
+@functools.lru_cache(maxsize=4096)
+def _row_major_configuration(shape: Tuple[int, ...]) -> NDConfiguration:
+    """The common case with the shape alone as the key (an enumeration's hash is computed in Python)."""
+    return _dense_configuration(shape, Layout.ROW_MAJOR)
