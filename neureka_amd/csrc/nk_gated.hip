@@ -109,22 +109,28 @@ struct Share {
 #pragma unroll
             for (int e = 0; e < E; e++) v[SET][e] = WHOLE || l + e < inner ? row[(int64_t)(l + e) * (ALONG ? 1 : ld)] : T(0);
     }
-    // LDS: fragments of 16 rows x 4 l, in the order in which the lanes of a wavefront hold them
+    // LDS: fragments of 16 rows x 4 l, in the order in which the lanes of a wavefront hold them; in every other fragment along l the
+    // neighbouring l change places, so that lanes that write one row do not meet in one bank
+    static __device__ __forceinline__ constexpr int turned(int k4) { return (k4 ^ (k4 >> 1)) & 1; }
     template <int SET>
     __device__ __forceinline__ void store(T* lds, int t) const {
         const int r = row_of(t), l = l_of(t);
 #pragma unroll
-        for (int e = 0; e < E; e++) lds[((r >> 4) * (BK / 4) + ((l + e) >> 2)) * 64 + ((l + e) & 3) * 16 + (r & 15)] = v[SET][e];
+        for (int e = 0; e < E; e++) {
+            const int k4 = (l + e) >> 2;
+            lds[((r >> 4) * (BK / 4) + k4) * 64 + (((l + e) & 3) ^ turned(k4)) * 16 + (r & 15)] = v[SET][e];
+        }
     }
 };
 
-// F x F fragments of 16 x 16 per wavefront, 4 wavefronts: tiles of 128 x 128 (F = 4) or 64 x 64, slices of 16 l in two LDS buffers.  f64,
-// F = 4: 64 x 64 x 16 multiply-adds are 16 x 4 matrix instructions against 32 LDS reads of 8 bytes a lane.
-template <typename T, int F, bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
-__global__ __launch_bounds__(256) void product_kernel(const Product<T> g) {
+// The f64 products: tiles of 64 x 64, 4 wavefronts of F x F fragments of 16 x 16, slices of 16 l in two LDS buffers; a wavefront's slice
+// is 16 matrix instructions of 64 cycles against 16 LDS reads of 8 bytes a lane.  52 TFLOP/s at 2048^3 (forward); tiles of 128 x 128 (two
+// blocks per unit, some registers spilled) 50 there, and half as fast from 1024^3 down, where there are too few of them.
+template <typename T, bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
+__global__ __launch_bounds__(256, 3) void product_kernel(const Product<T> g) {
     typedef Quad<T> Q;
     typedef typename Q::Acc Acc;
-    constexpr int BM = 32 * F, BN = 32 * F, BK = 16;
+    constexpr int F = 2, BM = 32 * F, BN = 32 * F, BK = 16;
     __shared__ T a_lds[2][BM * BK], b_lds[2][BN * BK];
     const unsigned tiles = (unsigned)(g.tiles_m * g.tiles_n), part = blockIdx.x / tiles;
     int tm, tn;
@@ -155,9 +161,10 @@ __global__ __launch_bounds__(256) void product_kernel(const Product<T> g) {
     };
     Acc acc[F][F] = {};
     const auto multiply = [&](int buffer) {
-        const T *const ap = a_lds[buffer] + lane, *const bp = b_lds[buffer] + lane;
 #pragma unroll
         for (int k = 0; k < BK / 4; k++) {
+            const int at = lane ^ (a.turned(k) * 16);
+            const T *const ap = a_lds[buffer] + at, *const bp = b_lds[buffer] + at;
             T af[F], bf[F];
 #pragma unroll
             for (int i = 0; i < F; i++) af[i] = ap[((wm * F + i) * (BK / 4) + k) * 64];
@@ -961,10 +968,10 @@ __global__ __launch_bounds__(256) void gated_errors_kernel(int fun, int64_t n, c
 // ---- plans ---------------------------------------------------------------------------------------------------------------
 struct Split { int edge_m, edge_n, tiles_m, tiles_n, parts, steps_per_part; };
 // What a slice of 16 l takes in the kernels of one tile size, in microseconds, and the blocks of it that a unit runs at a time (two planes;
-// with three every entry is near twice as long, which changes no choice): from 2048 x 1024 x 4096 and 4096^3, whole rounds.
+// with three every entry is near twice as long, which changes no choice): from 2048 x 1024 x 4096 and 4096^3, whole rounds; f64 512 x 512 x 2048.
 struct TileCost { int edge_m, edge_n, per_unit; double slice_us; };
 template <typename T> constexpr TileCost TILE_COSTS[] = {{256, 256, 1, 1.6}, {256, 128, 1, 0.92}, {128, 128, 2, 1.05}};
-template <> constexpr TileCost TILE_COSTS<double>[] = {{128, 128, 1, 3.0}, {64, 64, 3, 2.4}};
+template <> constexpr TileCost TILE_COSTS<double>[] = {{64, 64, 3, 2.4}};
 
 // The tile size and the number of parts of the contraction with the shortest estimate: rounds of blocks times slices, plus, with parts, a
 // launch that reads them all and writes the sum.
@@ -1010,9 +1017,8 @@ static void launch_tiles(Device* dev, const Product<float>& g, const Split& s, d
     if (g.a_scale) go(std::true_type()); else go(std::false_type());
 }
 template <bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
-static void launch_tiles(Device* dev, const Product<double>& g, const Split& s, dim3 grid) {
-    if (s.edge_m == 128) hipLaunchKernelGGL((product_kernel<double, 4, A_ALONG, B_ALONG, PAIRED, EPI>), grid, dim3(256), 0, dev->stream, g);
-    else               hipLaunchKernelGGL((product_kernel<double, 2, A_ALONG, B_ALONG, PAIRED, EPI>), grid, dim3(256), 0, dev->stream, g);
+static void launch_tiles(Device* dev, const Product<double>& g, const Split&, dim3 grid) {
+    hipLaunchKernelGGL((product_kernel<double, A_ALONG, B_ALONG, PAIRED, EPI>), grid, dim3(256), 0, dev->stream, g);
 }
 
 template <typename T, bool PAIRED, int EPI>

@@ -335,7 +335,9 @@ static int forward(Device* dev, const NormArgs<T>& a) {
     const int64_t cus = dev->props.multiProcessorCount;
     const bool held = with_row_plan<T>(a.cols, [&](auto block, auto threads, auto nv) {
         constexpr int BLOCK = decltype(block)::value, THREADS = decltype(threads)::value, NV = decltype(nv)::value, GROUPS = BLOCK / THREADS;
-        const int64_t all = (a.rows + GROUPS - 1) / GROUPS, most = cus * (2048 / BLOCK);
+        // blocks that stay and walk over the rows: with four vectors a thread 1024 threads per unit (4096 x 4096 floats 26.1 us, 2048 threads
+        // 27.6), with fewer 2048 (2047 x 1111 8.4, 1024 threads 8.8)
+        const int64_t all = (a.rows + GROUPS - 1) / GROUPS, most = cus * ((NV < 4 ? 2048 : 1024) / BLOCK);
         hipLaunchKernelGGL((norm_forward_kernel<T, BLOCK, THREADS, NV>), dim3((unsigned)(all < most ? all : most)), dim3(BLOCK), 0, dev->stream, a);
     });
     if (!held) hipLaunchKernelGGL((norm_forward_long_kernel<T>), dim3((unsigned)(a.rows < 2 * cus ? a.rows : 2 * cus)), dim3(1024), 0, dev->stream, a);
