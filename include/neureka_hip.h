@@ -259,7 +259,7 @@ int nk_fused(nk_dev dev, const int32_t* program, int n_ops, const double* consts
 /* Layer normalisation of `rows` rows of `cols` elements; row i of `src` starts at element i * src_pitch (src_pitch >= cols).
  *     drn = (src - mean) * rstd * gain + bias,  rstd = 1 / sqrt(variance + epsilon)  (gain and bias: `cols` elements each)
  * mean and rstd (`rows` elements each, both or neither 0) are written for the backward pass.  drn may be src where
- * src_pitch == cols. */
+ * src_pitch == cols.  cols <= 2^27 - 1024. */
 int nk_layer_norm(nk_dev dev, int dtype, int64_t rows, int64_t cols, nk_buf src, int64_t src_pitch, nk_buf gain, nk_buf bias,
                   double epsilon, nk_buf drn, nk_buf mean, nk_buf rstd);
 /* Its gradients for the error of drn: d_src (dense, rows x cols), d_gain and d_bias (`cols` elements); any of them may be 0
@@ -279,10 +279,17 @@ int nk_dropout(nk_dev dev, int dtype, int rank, nk_buf drn, const int32_t* drn_c
  *     gate = X @ Wg,  up = X @ Wu,  drn = f(gate) * up      X[M,K], Wg and Wu [K,N], drn[M,N]
  * f is one of NK_FUN_IDY, RELU, SIG, SILU, GELU, TANH.  weight_layout: NK_LAYOUT_ROW_MAJOR, or NK_LAYOUT_COLUMN_MAJOR for weights
  * stored as [N,K]; everything else is row-major.  gate and up ([M,N], both or neither 0) are written for the backward pass.
- * Element types: f64 products run on the f64 matrix cores.  f32 operands enter the matrix cores as sums of three bfloat16 numbers
- * (24 bits, exactly the operand's where its magnitude is 2^-110 or more), every product as the six partial products above
- * 2^-24 of it, added in f32: the error stays within 1e-5 of sum_k |x_ik| |w_kj| like that of nk_matmul, and infinities and NaN
- * give what f32 arithmetic gives.  Every sum is added in an order that depends on shape and layout alone. */
+ * f64 products run on the f64 matrix cores, f32 products of up to 32 rows (64 where the weights are small) on those of f32.  Larger
+ * f32 products take the 16-bit matrix cores in one of two ways, whichever is estimated to be faster, and add in f32:
+ *   - operands as sums of three bfloat16 numbers (24 bits, exactly the operand's where its magnitude is 2^-110 or more), every product
+ *     as its six partial products above 2^-24 of it;
+ *   - operands as sums of two half-precision numbers after a power of two per row of X and per column of a weight: 2^-16 of the largest
+ *     magnitude of that row or column or more keeps 22 bits and a sign, smaller numbers are off by at most 2^-40 of the largest.
+ *     Rows and columns below an outlier or spread over more than 24 binades, and any with an infinity or NaN, are found beforehand
+ *     and take the first way.
+ * The error stays within 1e-5 of sum_k (|x_ik| + 2^-23 X_i) (|w_kj| + 2^-23 W_j), X_i and W_j the largest magnitudes of row i of X
+ * and column j of W (the first way: within 1e-5 of sum_k |x_ik| |w_kj|, like nk_matmul); infinities, NaN and overflow give what f32
+ * arithmetic gives.  Every sum is added in an order that shape, layout and alignment fix.  M, K, N <= 2^27 - 1024. */
 int nk_gated_matmul(nk_dev dev, int fun_id, int dtype, int weight_layout, int64_t M, int64_t K, int64_t N, nk_buf X, nk_buf Wg, nk_buf Wu,
                     nk_buf drn, nk_buf gate, nk_buf up);
 /* Its gradients for the error of drn ([M,N]), with gate and up of the forward call:

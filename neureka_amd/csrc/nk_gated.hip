@@ -3,11 +3,16 @@
 //     gate = X Wg      up = X Wu      H = f(gate) up
 //     with the error E of H:  dg = E up f'(gate)   du = E f(gate)   dX = dg Wg^T + du Wu^T   dWg = X^T dg   dWu = X^T du
 //
-// All products are one kernel, result(m, n) = sum over l of A(m, l) B(n, l), on tiles of the result whose operands pass through
-// LDS.  Two switches say where an operand's neighbours along l lie (next to each other, or a row apart), which covers X, its
-// transpose and weights of either layout without a copy.  Two products that share A (forward, weight gradients) are
-// PAIRED: a tile holds the same columns of both, half each, so that A is staged once for both and f(gate) up is formed in the
-// registers that hold the sums.  dX is one product over a contraction of two segments, (dg, Wg) and then (du, Wu).
+// Every product is result(m, n) = sum over l of A(m, l) B(n, l).  Two switches say where an operand's neighbours along l lie (next to each
+// other, or a row apart), which covers X, its transpose and weights of either layout without a copy.  Two products that share A
+// (forward, weight gradients) are PAIRED: a tile holds the same columns of both, half each, so that A is staged once for both and
+// f(gate) up is formed in the registers that hold the sums.  dX is one product over a contraction of two segments, (dg, Wg) and then
+// (du, Wu).  What bounds them and what runs:
+//   few_rows_kernel        up to 32 rows (64 with few weights or in f64): the weights' bytes; straight from memory into registers
+//   split_product_kernel   f32: the 16-bit matrix cores, which take floats as sums of 16-bit numbers; tiles through LDS
+//   product_kernel         f64: the f64 matrix cores; tiles through LDS
+//   product_join_kernel    adds parts of the contraction where tiles alone would not fill the chip
+//   gated_errors_kernel    dg and du, once, for the three products of the backward pass
 #include "nk_internal.h"
 #include "nk_scalar.h"
 
@@ -246,8 +251,11 @@ __global__ __launch_bounds__(256, 3) void product_kernel(const Product<T> g) {
 // and x1 y1 is at most 2^-22 of x y (2^-25 on average, of either sign), as long as they stay within the type's few binades.
 // So a launch before finds, for every row of A and of B, the power of two that brings its largest magnitude below
 // 2^15; what is 2^-16 of that or more keeps all its bits, and smaller numbers are off by at most 2^-40 of the largest.
-// A row where that could show -- more than a quarter of its 64 stretches hold nothing beyond 2^-16 of the largest (and are not all
-// zero), or an infinity or NaN -- is marked, and tiles with a marked row take three planes.
+// A row where that could show is marked, and tiles with a marked row take three planes: one with an infinity or NaN, or where in more
+// than a quarter of those of its 64 stretches that are not all zero either everything is below 2^-16 of the largest or something other
+// than zero below 2^-24.  The first is an outlier above the row, the second a spread that the other operand may undo (columns of X scaled
+// one way, rows of a weight the other), where a small number counts as much as a large one.  Normally distributed numbers
+// have one element in 10^6 below 2^-24 of the largest, so rows of them are not marked.
 constexpr int MARKED = 1 << 30;                              // in place of a row's exponent
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -293,17 +301,27 @@ template <> struct Partial<2> {
 };
 
 // The exponents of up to five operands' rows (`count` rows of `length`, together with those of a second matrix where there is
-// one), blocks dealt out operand by operand.  Rows that lie along memory: a wavefront each, 64 stretches of every 64th 4
-// elements.  Rows across memory: 32 of them per block, 64 stretches of every 64th element.  Read once at memory speed.
+// one), blocks dealt out operand by operand.  Rows that lie along memory: a wavefront each, 64 stretches of every 64th 4 elements.
+// Rows across memory: 32 of them per block, 64 stretches of every 64th element.  Bound by memory: three operands of 4096 x 4096 in
+// 50 us, 4.0 TB/s.
 struct ScaleJob { const float* p[2]; int64_t ld; int count, length; bool along; int* out; unsigned blocks; };
 struct ScaleJobs { ScaleJob job[5]; int n; };
-__device__ __forceinline__ unsigned magnitude(float x) { return __builtin_bit_cast(unsigned, x) & 0x7fffffffu; }
-__device__ __forceinline__ int exponent_for(unsigned largest, int low, int some) {      // low of some non-zero stretches are far below the largest
+struct Range {                                               // of the magnitudes of a stretch, as their bits
+    unsigned most = 0, below_least = ~0u;                   // the least other than zero, less one
+    __device__ __forceinline__ void add(float x) {
+        const unsigned u = __builtin_bit_cast(unsigned, x) & 0x7fffffffu;
+        most = u > most ? u : most;
+        below_least = u - 1 < below_least ? u - 1 : below_least;
+    }
+    __device__ __forceinline__ bool far_below(unsigned largest) const {
+        return most != 0 && ((most >> 23) + 16 < (largest >> 23) || (below_least >> 23) + 24 < (largest >> 23));
+    }
+};
+__device__ __forceinline__ int exponent_for(unsigned largest, int low, int some) {      // low of some stretches that are not all zero are far below the largest
     if (largest >= 0x7f800000u || 4 * low > some) return MARKED;
     const int e = 14 + 127 - (int)(largest >> 23);
     return largest == 0 ? 0 : e < 126 ? e : 126;
 }
-__device__ __forceinline__ bool far_below(unsigned m, unsigned largest) { return m != 0 && (m >> 23) + 16 < (largest >> 23); }
 
 __global__ __launch_bounds__(512) void operand_scales_kernel(const ScaleJobs jobs) {
     unsigned block = blockIdx.x;
@@ -314,7 +332,7 @@ __global__ __launch_bounds__(512) void operand_scales_kernel(const ScaleJobs job
     if (j.along) {
         const int row = (int)block * 8 + wave;
         if (row >= j.count) return;
-        unsigned m = 0;
+        Range m;
         for (int k = 0; k < 2; k++) {
             if (!j.p[k]) continue;
             const float* const at = j.p[k] + (int64_t)row * j.ld;
@@ -323,14 +341,14 @@ __global__ __launch_bounds__(512) void operand_scales_kernel(const ScaleJobs job
             for (; i + 4 <= j.length; i += 256) {
                 const f32x4 v = *(const f32x4_any*)(at + i);
 #pragma unroll
-                for (int e = 0; e < 4; e++) { const unsigned u = magnitude(v[e]); m = u > m ? u : m; }
+                for (int e = 0; e < 4; e++) m.add(v[e]);
             }
-            for (; i < j.length; i++) { const unsigned u = magnitude(at[i]); m = u > m ? u : m; }
+            for (; i < j.length; i++) m.add(at[i]);
         }
-        unsigned largest = m;
+        unsigned largest = m.most;
 #pragma unroll
         for (int step = 32; step > 0; step >>= 1) { const unsigned o = __shfl_xor(largest, step); largest = o > largest ? o : largest; }
-        const int low = __popcll(__ballot(far_below(m, largest))), some = __popcll(__ballot(m != 0));
+        const int low = __popcll(__ballot(m.far_below(largest))), some = __popcll(__ballot(m.most != 0));
         if (lane == 0) j.out[row] = exponent_for(largest, low, some);
         return;
     }
@@ -338,7 +356,7 @@ __global__ __launch_bounds__(512) void operand_scales_kernel(const ScaleJobs job
     __shared__ unsigned waves_largest[8][32];
     __shared__ unsigned waves_low[8][8], waves_some[8][8];          // counts of 4 rows, a byte each
     const int q = lane & 7, c = (int)block * 32 + q * 4, first = wave * 8 + (lane >> 3);
-    unsigned m[4] = {0, 0, 0, 0};
+    Range m[4];
     for (int k = 0; k < 2; k++) {
         if (!j.p[k]) continue;
         if (c + 4 <= j.count) {
@@ -347,14 +365,14 @@ __global__ __launch_bounds__(512) void operand_scales_kernel(const ScaleJobs job
             for (int l = first; l < j.length; l += 64) {
                 const f32x4 v = *(const f32x4_any*)(at + (int64_t)l * j.ld);
 #pragma unroll
-                for (int e = 0; e < 4; e++) { const unsigned u = magnitude(v[e]); m[e] = u > m[e] ? u : m[e]; }
+                for (int e = 0; e < 4; e++) m[e].add(v[e]);
             }
         } else
             for (int l = first; l < j.length; l += 64)
 #pragma unroll
-                for (int e = 0; e < 4; e++) if (c + e < j.count) { const unsigned u = magnitude(j.p[k][(int64_t)l * j.ld + c + e]); m[e] = u > m[e] ? u : m[e]; }
+                for (int e = 0; e < 4; e++) if (c + e < j.count) m[e].add(j.p[k][(int64_t)l * j.ld + c + e]);
     }
-    unsigned largest[4] = {m[0], m[1], m[2], m[3]};
+    unsigned largest[4] = {m[0].most, m[1].most, m[2].most, m[3].most};
 #pragma unroll
     for (int step = 8; step < 64; step <<= 1)
 #pragma unroll
@@ -367,8 +385,8 @@ __global__ __launch_bounds__(512) void operand_scales_kernel(const ScaleJobs job
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         for (int w = 0; w < 8; w++) { const unsigned o = waves_largest[w][q * 4 + e]; largest[e] = o > largest[e] ? o : largest[e]; }
-        low |= (unsigned)far_below(m[e], largest[e]) << (8 * e);
-        some |= (unsigned)(m[e] != 0) << (8 * e);
+        low |= (unsigned)m[e].far_below(largest[e]) << (8 * e);
+        some |= (unsigned)(m[e].most != 0) << (8 * e);
     }
 #pragma unroll
     for (int step = 8; step < 64; step <<= 1) { low += __shfl_xor(low, step); some += __shfl_xor(some, step); }
@@ -463,6 +481,12 @@ struct SplitShare {
     }
 };
 
+// Three tile sizes: 256 x 256 (8 wavefronts of 128 x 64: 48 KiB of LDS reads for 48 matrix instructions of a slice), 256 x 128 and
+// 128 x 128.  4096^3 forward, two planes: 756 us, 1.09e15 operations on halves a second, 364 TFLOP/s of float products (the f32
+// instruction's peak is 157, a library's product of floats reaches 154).  The clock falls to 1.7 GHz under it with the matrix cores busy 61 %
+// of the cycles, as under any dense product of 16-bit numbers here (a library's product of bfloat16, 8192^3: 1.3e15); without the
+// requests to memory and the splitting the same loop takes 605 us.  Three planes: 1199 us.
+//
 // WM x WN wavefronts, each with a tile of FI x FJ fragments of 32 x 32.  PAIRED: the first half of a wavefront's column
 // fragments comes from the first product, the second half from the second.
 template <int PLANES, int WM, int WN, int FI, int FJ, bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
@@ -900,7 +924,8 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int p
 }
 
 // ---- parts of the contraction, added in order -----------------------------------------------------------------------
-// partial: [parts][halves][n]; halves 2: the pair of products.  Four elements a thread.
+// partial: [parts][halves][n]; halves 2: the pair of products.  Four elements a thread; bound by memory (4 parts of 2048 x 1024
+// floats 8 us, 5 TB/s).
 template <typename T, bool PAIRED, int EPI>
 __global__ __launch_bounds__(256) void product_join_kernel(const T* __restrict__ partial, int parts, int64_t n, int fun, T* out0, T* out1, T* out2) {
     typedef T V __attribute__((ext_vector_type(4), aligned(sizeof(T))));
@@ -938,7 +963,7 @@ __global__ __launch_bounds__(256) void product_join_kernel(const T* __restrict__
     }
 }
 
-// dg = E up f'(gate), du = E f(gate): five numbers through memory per element, four elements a thread
+// dg = E up f'(gate), du = E f(gate): five numbers through memory per element, four elements a thread (4096 x 4096 floats 57 us, 5.9 TB/s)
 template <typename T>
 __global__ __launch_bounds__(256) void gated_errors_kernel(int fun, int64_t n, const T* __restrict__ error, const T* __restrict__ gate, const T* __restrict__ up,
                                                            T* __restrict__ d_gate, T* __restrict__ d_up) {
@@ -1198,9 +1223,9 @@ static int check_gated(const char* what, int fun, int dtype, int layout, int64_t
     NK_REQUIRE(fun == NK_FUN_IDY || fun == NK_FUN_RELU || fun == NK_FUN_SIG || fun == NK_FUN_SILU || fun == NK_FUN_GELU || fun == NK_FUN_TANH,
                "%s: function id %d is none of idy, relu, sig, silu, gelu, tanh", what, fun);
     NK_REQUIRE(layout == NK_LAYOUT_ROW_MAJOR || layout == NK_LAYOUT_COLUMN_MAJOR, "%s: unknown layout %d", what, layout);
-    const int64_t most = (int64_t)1 << 31, longest = most - 1024;       // (a tile past the end of an axis still counts in 32 bits)
+    const int64_t most = (int64_t)1 << 31, longest = ((int64_t)1 << 27) - 1024;       // (512 threads for 16 of an axis stay below the 2^32 of a launch)
     NK_REQUIRE(M >= 1 && K >= 1 && N >= 1, "%s: M, K, N must be positive (got %lld, %lld, %lld)", what, (long long)M, (long long)K, (long long)N);
-    NK_REQUIRE(M <= longest && K <= longest && N <= longest && M * K < most && K * N < most && M * N < most, "%s: operands are limited to 2^31-1 elements and axes to 2^31-1024", what);
+    NK_REQUIRE(M <= longest && K <= longest && N <= longest && M * K < most && K * N < most && M * N < most, "%s: operands are limited to 2^31-1 elements and axes to 2^27-1024", what);
     return NK_OK;
 }
 struct Piece { const char* name; nk_buf at; uint64_t bytes; };

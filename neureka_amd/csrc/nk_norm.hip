@@ -386,7 +386,8 @@ static bool overlap(nk_buf a, uint64_t n, nk_buf b, uint64_t m) { return a && b 
 static int check_rows(const char* what, int dtype, int64_t rows, int64_t cols, int64_t pitch) {
     NK_REQUIRE(dtype == NK_F32 || dtype == NK_F64, "%s: unknown dtype %d", what, dtype);
     NK_REQUIRE(rows >= 1 && cols >= 1, "%s: rows and columns must be positive (got %lld, %lld)", what, (long long)rows, (long long)cols);
-    NK_REQUIRE(cols <= ((int64_t)1 << 31) - 2048, "%s: rows of %lld elements, 2^31-2048 are the most", what, (long long)cols);      // (a step past the end still counts in 32 bits)
+    // (norm_add_shares_kernel's 16 threads per column stay below the 2^32 of a launch)
+    NK_REQUIRE(cols <= ((int64_t)1 << 27) - 1024, "%s: rows of %lld elements, 2^27-1024 are the most", what, (long long)cols);
     NK_REQUIRE(rows < ((int64_t)1 << 31) && rows * cols < ((int64_t)1 << 31), "%s: %lld x %lld exceeds 2^31-1 elements", what, (long long)rows, (long long)cols);
     NK_REQUIRE(pitch >= cols && pitch < ((int64_t)1 << 31), "%s: a pitch of %lld elements does not hold rows of %lld", what, (long long)pitch, (long long)cols);
     return NK_OK;

@@ -615,3 +615,52 @@ def test_large_gated_infinities_and_nan(device):
             ok = np.isfinite(want)
             amount = np.abs(np.where(np.isfinite(X), X, 0)) @ np.abs(np.where(np.isfinite(W), W, 0))
             within(got[ok], want[ok], sum_roundings(K) * unit(np.float32) * amount[ok], "finite ones")
+
+
+@pytest.mark.parametrize("along", [False, True])
+@pytest.mark.parametrize("spread", [12, 40])
+def test_large_gated_scales_that_undo_each_other(device, along, spread):
+    """The columns of x times powers of two, the rows of the weights divided by them: every product counts alike, the small entries of
+    either operand no less than the large ones."""
+    rng = np.random.default_rng(23)
+    M, K, N = 1200, 1400, 1310
+    by = 2.0 ** rng.integers(-spread, spread + 1, K)
+    x = (rng.standard_normal((M, K)) * by).astype(np.float32)
+    wg, wu = ((rng.standard_normal((K, N)) / by[:, None]).astype(np.float32) for _ in range(2))
+    for got, w in zip(rows_of(device, x, wg, wu, along), (wg, wu)):
+        X, W = x.astype(np.float64), w.astype(np.float64)
+        within(got, X @ W, sum_roundings(K) * unit(np.float32) * (np.abs(X) @ np.abs(W)), "gate or up")
+
+
+def test_large_gated_gradients_with_scales_that_undo_each_other(device):
+    """The same for d_X (columns of the weights against those of the error) and the weights' gradients (rows of x against those of
+    the error), with the products as plain factors."""
+    rng = np.random.default_rng(24)
+    M, K, N = 1200, 1400, 1310
+    one = device.allocateFromOne(np.float32, M * N, 1.0)      # gate = up = 1, the identity: dg = du = error
+    for axis in (0, 1):
+        by = 2.0 ** rng.integers(-40, 41, (M, 1) if axis == 0 else (1, N))
+        x = (rng.standard_normal((M, K)) * (by if axis == 0 else 1)).astype(np.float32)
+        wg, wu = ((rng.standard_normal((K, N)) * (by if axis == 1 else 1)).astype(np.float32) for _ in range(2))
+        e = (rng.standard_normal((M, N)) / by).astype(np.float32)
+        X, G, U, E = (a.astype(np.float64) for a in (x, wg, wu, e))
+        d_x, d_g, d_u = (put(device, np.zeros(s, np.float32)) for s in ((M, K), (K, N), (K, N)))
+        device.launch_gated_matmul_backward("idy", put(device, x), put(device, wg), put(device, wu), one, one, put(device, e), d_x, d_g, d_u)
+        r = unit(np.float32)
+        within(get(d_x), E @ (G + U).T, sum_roundings(2 * N) * r * (np.abs(E) @ (np.abs(G) + np.abs(U)).T), "dX")
+        for got in (d_g, d_u):
+            within(get(got), X.T @ E, sum_roundings(M) * r * (np.abs(X.T) @ np.abs(E)), "dW")
+
+
+def test_axes_beyond_a_launch_are_refused(device):
+    """A launch has fewer than 2^32 threads: axes that would need more are refused, whatever the buffers hold."""
+    from neureka_amd._lib import FUN
+    lib, h, p = device._lib, device.handle, put(device, np.zeros(4, np.float32))._data.ptr
+    for axis in range(3):
+        axes = [1, 1, 1]
+        axes[axis] = (1 << 27) - 1023
+        for dt in (0, 1):
+            assert lib.nk_gated_matmul(h, FUN["silu"], dt, 0, *axes, p, p, p, p, 0, 0) != 0
+            assert b"2^27" in lib.nk_last_error()
+    assert lib.nk_layer_norm(h, 0, 1, (1 << 27) - 1023, p, 1 << 27, p, p, 1e-5, p, 0, 0) != 0
+    assert b"2^27" in lib.nk_last_error()
