@@ -122,6 +122,39 @@ public final class Hip {
         Nk.check(() -> (int) Nk.nk_reduce_index.invokeExact(dev.handle, kind, HipDevice.dtype(in.itemType()), HipDevice.ptr(in), (long) in.size(), HipDevice.ptr(index)));
         return index;                                                         // Min.java reads index.item(0) and wraps in.item(i)
     }
+    // ---- the operators of a feed-forward sublayer (no counterpart in the reference): dense row-major tensors; a gradient that is not wanted is null
+    private static long at(Tensor<?> t) { return t == null ? 0L : HipDevice.ptr(t); }
+    /** drn = (src - mean) * rstd * gain + bias over the last axis; mean and rstd (one item per row) are kept for the backward pass, or both null. */
+    public static void layerNorm(HipDevice dev, Tensor<?> drn, Tensor<?> src, Tensor<?> gain, Tensor<?> bias, double epsilon, Tensor<?> mean, Tensor<?> rstd) {
+        long cols = src.shape(src.rank() - 1), rows = src.size() / cols;
+        Nk.check(() -> (int) Nk.nk_layer_norm.invokeExact(dev.handle, HipDevice.dtype(src.itemType()), rows, cols, at(src), cols, at(gain), at(bias),
+                                                         epsilon, at(drn), at(mean), at(rstd)));
+    }
+    public static void layerNormBackward(HipDevice dev, Tensor<?> src, Tensor<?> gain, Tensor<?> mean, Tensor<?> rstd, Tensor<?> error,
+                                         Tensor<?> dSrc, Tensor<?> dGain, Tensor<?> dBias) {
+        long cols = src.shape(src.rank() - 1), rows = src.size() / cols;
+        Nk.check(() -> (int) Nk.nk_layer_norm_backward.invokeExact(dev.handle, HipDevice.dtype(src.itemType()), rows, cols, at(src), cols, at(gain), at(mean),
+                                                                  at(rstd), at(error), at(dSrc), at(dGain), at(dBias)));
+    }
+    /** drn = keep ? src / (1 - probability) : 0; the backward pass is the same call on the error.  Any view. */
+    public static void dropout(HipDevice dev, Tensor<?> drn, Tensor<?> src, double probability, long seed, long offset) {
+        try (Arena a = Arena.ofConfined()) {
+            MemorySegment c0 = Nk.cfg(a, drn), c1 = Nk.cfg(a, src);
+            Nk.check(() -> (int) Nk.nk_dropout.invokeExact(dev.handle, HipDevice.dtype(drn.itemType()), drn.rank(), at(drn), c0, at(src), c1,
+                                                          probability, seed, offset, (long) drn.size()));
+        }
+    }
+    /** drn = f(x @ gateWeight) * (x @ upWeight); weights [K,N], byColumns: stored [N,K]; both products are kept for the backward pass, or both null. */
+    public static void gatedMatMul(HipDevice dev, ScalarFun f, boolean byColumns, long K, long N, Tensor<?> drn, Tensor<?> x, Tensor<?> gateWeight, Tensor<?> upWeight,
+                                   Tensor<?> gate, Tensor<?> up) {
+        Nk.check(() -> (int) Nk.nk_gated_matmul.invokeExact(dev.handle, funId(f), HipDevice.dtype(x.itemType()), byColumns ? 1 : 0, x.size() / K, K, N,
+                                                           at(x), at(gateWeight), at(upWeight), at(drn), at(gate), at(up)));
+    }
+    public static void gatedMatMulBackward(HipDevice dev, ScalarFun f, boolean byColumns, long K, long N, Tensor<?> x, Tensor<?> gateWeight, Tensor<?> upWeight,
+                                           Tensor<?> gate, Tensor<?> up, Tensor<?> error, Tensor<?> dX, Tensor<?> dGateWeight, Tensor<?> dUpWeight) {
+        Nk.check(() -> (int) Nk.nk_gated_matmul_backward.invokeExact(dev.handle, funId(f), HipDevice.dtype(x.itemType()), byColumns ? 1 : 0, x.size() / K, K, N,
+                                                                    at(x), at(gateWeight), at(upWeight), at(gate), at(up), at(error), at(dX), at(dGateWeight), at(dUpWeight)));
+    }
     /** One launch of nk_fused: program / consts as HipFunctionCompiler lowers them (CLFunctionCompiler.java:101-199). */
     public static Tensor<?> fused(HipDevice dev, int[] program, double[] consts, Tensor<?> drn, Tensor<?>[] srcs) {
         try (Arena a = Arena.ofConfined()) {
