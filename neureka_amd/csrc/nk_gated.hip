@@ -83,158 +83,167 @@ __device__ __forceinline__ void own_tile(unsigned block, unsigned tiles, int til
     tn = (int)(in / height);
 }
 
-__device__ __forceinline__ void lds_barrier() {             // orders LDS only: requests to memory stay in flight
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
-// One operand's share of a slice: `WIDTH` rows of the result (or columns, for B) by 16 steps of l, 256 threads, E consecutive l
-// each; two slices on their way.
-template <typename T, int WIDTH, bool ALONG>
-struct Share {
-    static constexpr int BK = 16, E = WIDTH * BK / 256, PER_ROW = BK / E, V = 16 / sizeof(T);
-    T v[2][E];
-    static __device__ __forceinline__ int row_of(int t) { return ALONG ? t / PER_ROW : t % WIDTH; }
-    static __device__ __forceinline__ int l_of(int t) { return ALONG ? (t % PER_ROW) * E : __builtin_amdgcn_readfirstlane(t / WIDTH) * E; }
-    // `row`: the operand's first element of this thread's row; `l0`: the slice's first l.  WHOLE: all 16 l of the slice exist; else what
-    // lies past `inner` is zero.
-    template <int SET, bool WHOLE>
-    __device__ __forceinline__ void load(const T* row, int64_t ld, int l0, int inner, int t) {
-        const int l = l0 + l_of(t);
-        if constexpr (ALONG && WHOLE) {
-            typedef T Vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+// The f64 products: tiles of 64 x 64, the contraction shared by the block's 4 wavefronts, steps of 16 l in turn.  Every wavefront holds the
+// whole tile (4 x 4 fragments of 16 x 16) and nothing it reads is another's, so its operands go from memory straight into the
+// registers of the matrix instructions: 32 instructions of 64 cycles to a chunk of 8 l, whose eight 16-byte loads went out a chunk
+// before.  No barrier until the sums meet in LDS, where each wavefront takes a quarter of the tile.
+//
+// Quarter q of a wavefront takes l = 2 q, 2 q + 1 of a chunk.  Operands that lie along l: a lane's two values are one load.  Operands that
+// lie across: a lane loads two neighbouring rows (columns) of one l, so fragments 2 h and 2 h + 1 hold rows 32 h + 2 r and 32 h + 2 r + 1.
+template <bool ALONG>
+struct Strip {                                              // 64 rows of A (columns of B); PAIRED: 32 of either of two matrices
+    const double* at[4];                                    // ALONG: a row each; across: the first of two, at[h] (from l = 2 q on either way)
+    // `first[h]`: the row at which 32 rows of the strip start; rows past the end are read as the last ones, which the store leaves out
+    __device__ __forceinline__ void place(const double* const (&from)[2], const int (&first)[2], int count, int64_t ld, int lane) {
+        const int c = lane & 15, q = lane >> 4;
 #pragma unroll
-            for (int u = 0; u < E / V; u++) {
-                const Vec x = *(const Vec*)(row + l + u * V);
+        for (int h = 0; h < 2; h++) {
+            if constexpr (ALONG) {
 #pragma unroll
-                for (int e = 0; e < V; e++) v[SET][u * V + e] = x[e];
+                for (int e = 0; e < 2; e++) {
+                    const int r = first[h] + e * 16 + c;
+                    at[2 * h + e] = from[h] + (int64_t)(r < count ? r : count - 1) * ld + 2 * q;
+                }
+            } else at[h] = from[h] + pair_of(first[h] + 2 * c, count) + (int64_t)(2 * q) * ld;
+        }
+    }
+    static __device__ __forceinline__ int pair_of(int r, int count) { return r + 2 <= count ? r : count - 2; }
+    // the row of the strip's fragment f that index r of the fragment stands for, given the 32 rows' first; -1: none
+    static __device__ __forceinline__ int row_of(int first, int f, int r, int count) {
+        if constexpr (ALONG) { const int m = first + (f & 1) * 16 + r; return m < count ? m : -1; }
+        const int own = first + 2 * r, m = pair_of(own, count) + (f & 1);
+        return m >= own && m < count ? m : -1;
+    }
+    __device__ __forceinline__ void load(double (&v)[4][2], int64_t shift, int64_t ld, int l0) const {      // v[fragment][l]
+        typedef double V __attribute__((ext_vector_type(2), aligned(8)));
+        if constexpr (ALONG) {
+#pragma unroll
+            for (int f = 0; f < 4; f++) {
+                const V x = *(const V*)(at[f] + shift + l0);
+                v[f][0] = x[0]; v[f][1] = x[1];
             }
         } else
 #pragma unroll
-            for (int e = 0; e < E; e++) v[SET][e] = WHOLE || l + e < inner ? row[(int64_t)(l + e) * (ALONG ? 1 : ld)] : T(0);
-    }
-    // LDS: fragments of 16 rows x 4 l, in the order in which the lanes of a wavefront hold them; in every other fragment along l the
-    // neighbouring l change places, so that lanes that write one row do not meet in one bank
-    static __device__ __forceinline__ constexpr int turned(int k4) { return (k4 ^ (k4 >> 1)) & 1; }
-    template <int SET>
-    __device__ __forceinline__ void store(T* lds, int t) const {
-        const int r = row_of(t), l = l_of(t);
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            const int k4 = (l + e) >> 2;
-            lds[((r >> 4) * (BK / 4) + k4) * 64 + (((l + e) & 3) ^ turned(k4)) * 16 + (r & 15)] = v[SET][e];
-        }
+                for (int s = 0; s < 2; s++) {
+                    const V x = *(const V*)(at[h] + shift + (int64_t)(l0 + s) * ld);
+                    v[2 * h][s] = x[0]; v[2 * h + 1][s] = x[1];
+                }
+    }
+    // the same where the contraction ends inside the chunk: zero from `inner` on
+    __device__ __forceinline__ void load_rest(double (&v)[4][2], int64_t shift, int64_t ld, int l0, int inner, int lane) const {
+        const int l = l0 + 2 * (lane >> 4);
+#pragma unroll
+        for (int f = 0; f < 4; f++)
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+                v[f][s] = l + s < inner ? (ALONG ? at[f][shift + l0 + s] : at[f >> 1][shift + (int64_t)(l0 + s) * ld + (f & 1)]) : 0.0;
     }
 };
 
-// The f64 products: tiles of 64 x 64, 4 wavefronts of F x F fragments of 16 x 16, slices of 16 l in two LDS buffers; a wavefront's slice
-// is 16 matrix instructions of 64 cycles against 16 LDS reads of 8 bytes a lane.  52 TFLOP/s at 2048^3 (forward); tiles of 128 x 128 (two
-// blocks per unit, some registers spilled) 50 there, and half as fast from 1024^3 down, where there are too few of them.
-template <typename T, bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
-__global__ __launch_bounds__(256, 3) void product_kernel(const Product<T> g) {
-    typedef Quad<T> Q;
-    typedef typename Q::Acc Acc;
-    constexpr int F = 2, BM = 32 * F, BN = 32 * F, BK = 16;
-    __shared__ T a_lds[2][BM * BK], b_lds[2][BN * BK];
+template <bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
+__global__ __launch_bounds__(256, 2) void product_kernel(const Product<double> g) {
+    typedef Quad<double> Q;
+    typedef Q::Acc Acc;
+    constexpr int BM = 64, HALF = PAIRED ? 32 : 64, KC = 8, BK = 16;
+    __shared__ Acc sums[2][3][4][64];                       // two rows of fragments at a time, three wavefronts' shares
     const unsigned tiles = (unsigned)(g.tiles_m * g.tiles_n), part = blockIdx.x / tiles;
     int tm, tn;
     own_tile(blockIdx.x - part * tiles, tiles, g.tiles_m, g.tiles_n, tm, tn);
-    constexpr int HALF = PAIRED ? BN / 2 : BN;
     const int m0 = tm * BM, n0 = tn * HALF;
-    const int t = threadIdx.x, wave = t >> 6, lane = t & 63, wm = wave >> 1, wn = wave & 1;
-    Share<T, BM, A_ALONG> a;
-    Share<T, BN, B_ALONG> b;
-    // rows and columns past the end are read as the last one; what they give is not stored
-    const int64_t am = m0 + a.row_of(t) < g.rows ? m0 + a.row_of(t) : g.rows - 1;
-    const int bt = b.row_of(t), half = PAIRED ? bt / HALF : 0, bc = n0 + (PAIRED ? bt % HALF : bt);
-    const int64_t bn = bc < g.cols ? bc : g.cols - 1;
-    // whole slices of all segments first, g.steps_per_part of them per part; the last part also takes what is left of each segment
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int a_first[2] = {m0, m0 + 32}, b_first[2] = {n0, PAIRED ? n0 : n0 + 32};
+    Strip<A_ALONG> a;
+    Strip<B_ALONG> b;
+    const double *const a_from[2] = {g.A[0], g.A[0]}, *const b_from[2] = {g.B[0], PAIRED ? g.B[1] : g.B[0]};
+    a.place(a_from, a_first, g.rows, g.lda, lane);
+    b.place(b_from, b_first, g.cols, g.ldb, lane);
+    // whole steps of all segments first, g.steps_per_part of them per part; the last part also takes what is left of each segment
     const int whole = g.inner / BK, all = whole * g.segments;
     const int first = (int)part * g.steps_per_part < all ? (int)part * g.steps_per_part : all;
     const int last = first + g.steps_per_part < all ? first + g.steps_per_part : all;
-    const auto request = [&](auto set, auto complete, int segment, int l0) {
-        constexpr int SET = decltype(set)::value;
-        constexpr bool WHOLE = decltype(complete)::value;
-        a.template load<SET, WHOLE>(g.A[segment] + am * (A_ALONG ? g.lda : 1), g.lda, l0, g.inner, t);
-        b.template load<SET, WHOLE>(g.B[PAIRED ? half : segment] + bn * (B_ALONG ? g.ldb : 1), g.ldb, l0, g.inner, t);
-    };
-    const auto request_slice = [&](auto set, int s) {        // past the end: the last one once more
+    const int64_t a_shift = PAIRED ? 0 : g.A[1] - g.A[0], b_shift = PAIRED ? 0 : g.B[1] - g.B[0];       // to the second segment
+    struct Chunk { double a[4][2], b[4][2]; };
+    const auto request = [&](Chunk& k, int s, int half) {   // past the end: the last one once more
         s = s < last ? s : last - 1;
-        const int segment = s >= whole;
-        request(set, std::true_type(), segment, (s - segment * whole) * BK);
+        const bool second = !PAIRED && s >= whole;
+        const int l0 = (second ? s - whole : s) * BK + half * KC;
+        a.load(k.a, second ? a_shift : 0, g.lda, l0);
+        b.load(k.b, second ? b_shift : 0, g.ldb, l0);
     };
-    Acc acc[F][F] = {};
-    const auto multiply = [&](int buffer) {
+    Acc acc[4][4] = {};
+    const auto multiply = [&](const Chunk& k) {
 #pragma unroll
-        for (int k = 0; k < BK / 4; k++) {
-            const int at = lane ^ (a.turned(k) * 16);
-            const T *const ap = a_lds[buffer] + at, *const bp = b_lds[buffer] + at;
-            T af[F], bf[F];
+        for (int s = 0; s < 2; s++)
 #pragma unroll
-            for (int i = 0; i < F; i++) af[i] = ap[((wm * F + i) * (BK / 4) + k) * 64];
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int j = 0; j < F; j++) {
-                const int block = PAIRED ? (j / (F / 2)) * F + wn * (F / 2) + j % (F / 2) : wn * F + j;
-                bf[j] = bp[(block * (BK / 4) + k) * 64];
-            }
-#pragma unroll
-            for (int i = 0; i < F; i++)
-#pragma unroll
-                for (int j = 0; j < F; j++) acc[i][j] = Q::mma(af[i], bf[j], acc[i][j]);
+                for (int j = 0; j < 4; j++) acc[i][j] = Q::mma(k.a[i][s], k.b[j][s], acc[i][j]);
+    };
+    if (first + wave < last) {
+        Chunk one, two;
+        request(one, first + wave, 0);
+        for (int s = first + wave; s < last; s += 4) {
+            request(two, s, 1);
+            __builtin_amdgcn_sched_barrier(0);               // the requests go out before the products of the chunk that is here
+            multiply(one);
+            request(one, s + 4, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(two);
         }
-    };
-    typedef std::integral_constant<int, 0> Even;
-    typedef std::integral_constant<int, 1> Odd;
-    if (first < last) {
-        // slice s is in LDS, s + 1 and s + 2 in registers or on their way
-        request_slice(Even(), first);
-        request_slice(Odd(), first + 1);
-        a.template store<0>(a_lds[0], t); b.template store<0>(b_lds[0], t);
-        request_slice(Even(), first + 2);
-        lds_barrier();
-        const auto slice = [&](auto parity, int s) {
-            constexpr int P = decltype(parity)::value;
-            a.template store<1 - P>(a_lds[1 - P], t); b.template store<1 - P>(b_lds[1 - P], t);
-            request_slice(std::integral_constant<int, 1 - P>(), s + 3);
-            multiply(P);
-            lds_barrier();
-        };
-        int s = first;
-        for (; s + 1 < last; s += 2) { slice(Even(), s); slice(Odd(), s + 1); }
-        if (s < last) slice(Even(), s);
     }
-    if (g.inner % BK != 0 && last == all)
-        for (int segment = 0; segment < g.segments; segment++) {
-            request(Even(), std::false_type(), segment, whole * BK);
-            a.template store<0>(a_lds[0], t); b.template store<0>(b_lds[0], t);
-            lds_barrier();
-            multiply(0);
-            lds_barrier();
+    if (wave == 3 && g.inner % BK != 0 && last == all)
+        for (int segment = 0; segment < g.segments; segment++)
+            for (int l0 = whole * BK; l0 < g.inner; l0 += KC) {
+                Chunk rest;
+                a.load_rest(rest.a, segment ? a_shift : 0, g.lda, l0, g.inner, lane);
+                b.load_rest(rest.b, segment ? b_shift : 0, g.ldb, l0, g.inner, lane);
+                multiply(rest);
+            }
+    // row i of fragments belongs to wavefront i, which adds the shares of the others to its own in a fixed order
+#pragma unroll
+    for (int pass = 0; pass < 2; pass++) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int i = pass * 2 + e;
+            if (wave != i)
+#pragma unroll
+                for (int j = 0; j < 4; j++) sums[e][wave - (wave > i)][j][lane] = acc[i][j];
         }
+        __syncthreads();
+        if (wave >> 1 == pass)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                Acc x = wave & 1 ? acc[pass * 2 + 1][j] : acc[pass * 2][j];
+#pragma unroll
+                for (int w = 0; w < 3; w++) x += sums[wave & 1][w][j][lane];
+                acc[0][j] = x;                               // (its own share is not needed again, nor is row 0 of any other wavefront)
+            }
+        if (pass == 0) __syncthreads();
+    }
     const int64_t shift = (int64_t)part * g.part_stride;
+    const int c = lane & 15;
 #pragma unroll
-    for (int i = 0; i < F; i++)
+    for (int v = 0; v < 4; v++) {
+        const int m = a.row_of(m0 + (wave >> 1) * 32, wave, Q::row(lane, v), g.rows);
+        if (m < 0) continue;
+        const int64_t row = (int64_t)m * g.cols + shift;
 #pragma unroll
-        for (int v = 0; v < 4; v++) {
-            const int m = m0 + wm * (16 * F) + i * 16 + Q::row(lane, v);
-            if (m >= g.rows) continue;
-            const int64_t row = (int64_t)m * g.cols + shift;
-#pragma unroll
-            for (int j = 0; j < (PAIRED ? F / 2 : F); j++) {
-                const int n = n0 + (PAIRED ? wn * (8 * F) : wn * (16 * F)) + j * 16 + (lane & 15);
-                if (n >= g.cols) continue;
-                const T x = acc[i][j][v];
-                if constexpr (!PAIRED) g.out[0][row + n] = x;
-                else {
-                    const T y = acc[i][F / 2 + j % (F / 2)][v];
-                    if constexpr (EPI == GATED) {
-                        g.out[0][row + n] = gated_fun(g.fun, x) * y;
-                        if (g.out[1]) { g.out[1][row + n] = x; g.out[2][row + n] = y; }
-                    } else { g.out[0][row + n] = x; g.out[1][row + n] = y; }
-                }
+        for (int j = 0; j < (PAIRED ? 2 : 4); j++) {
+            const int n = b.row_of(n0 + (j >> 1) * 32, j, c, g.cols);
+            if (n < 0) continue;
+            const double x = acc[0][j][v];
+            if constexpr (!PAIRED) g.out[0][row + n] = x;
+            else {
+                const double y = acc[0][j + 2][v];
+                if constexpr (EPI == GATED) {
+                    g.out[0][row + n] = gated_fun(g.fun, x) * y;
+                    if (g.out[1]) { g.out[1][row + n] = x; g.out[2][row + n] = y; }
+                } else { g.out[0][row + n] = x; g.out[1][row + n] = y; }
             }
         }
+    }
 }
 
 // ---- f32 products on the 16-bit matrix cores --------------------------------------------------------------------------
@@ -399,6 +408,12 @@ __global__ __launch_bounds__(512) void operand_scales_kernel(const ScaleJobs job
         for (int e = 0; e < 4; e++)
             if (c + e < j.count) j.out[c + e] = exponent_for(largest[e], (low >> (8 * e)) & 255, (some >> (8 * e)) & 255);
     }
+}
+
+__device__ __forceinline__ void lds_barrier() {             // orders LDS only: requests to memory stay in flight
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // LDS holds an operand's slice (WIDTH rows x 16 l) as PLANES planes of fragments of 32 rows x 16 l in the order in which the
@@ -996,7 +1011,7 @@ struct Split { int edge_m, edge_n, tiles_m, tiles_n, parts, steps_per_part; };
 // with three every entry is near twice as long, which changes no choice): from 2048 x 1024 x 4096 and 4096^3, whole rounds; f64 512 x 512 x 2048.
 struct TileCost { int edge_m, edge_n, per_unit; double slice_us; };
 template <typename T> constexpr TileCost TILE_COSTS[] = {{256, 256, 1, 1.6}, {256, 128, 1, 0.92}, {128, 128, 2, 1.05}};
-template <> constexpr TileCost TILE_COSTS<double>[] = {{64, 64, 3, 2.4}};
+template <> constexpr TileCost TILE_COSTS<double>[] = {{64, 64, 2, 1.1}};
 
 // The tile size and the number of parts of the contraction with the shortest estimate: rounds of blocks times slices, plus, with parts, a
 // launch that reads them all and writes the sum.
@@ -1043,7 +1058,13 @@ static void launch_tiles(Device* dev, const Product<float>& g, const Split& s, d
 }
 template <bool A_ALONG, bool B_ALONG, bool PAIRED, int EPI>
 static void launch_tiles(Device* dev, const Product<double>& g, const Split&, dim3 grid) {
-    hipLaunchKernelGGL((product_kernel<double, A_ALONG, B_ALONG, PAIRED, EPI>), grid, dim3(256), 0, dev->stream, g);
+    // a matrix of one row lies along and across alike; taken as along, since the kernel reads what lies across by twos
+    const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, dev->stream, g); };
+    const bool a = A_ALONG || g.rows == 1, b = B_ALONG || g.cols == 1;
+    if (a && b)  run(product_kernel<true, true, PAIRED, EPI>);
+    else if (a)  run(product_kernel<true, false, PAIRED, EPI>);
+    else if (b)  run(product_kernel<false, true, PAIRED, EPI>);
+    else         run(product_kernel<false, false, PAIRED, EPI>);
 }
 
 template <typename T, bool PAIRED, int EPI>
