@@ -165,10 +165,11 @@ __global__ __launch_bounds__(256, 2) void product_kernel(const Product<double> g
     const int last = first + g.steps_per_part < all ? first + g.steps_per_part : all;
     const int64_t a_shift = PAIRED ? 0 : g.A[1] - g.A[0], b_shift = PAIRED ? 0 : g.B[1] - g.B[0];       // to the second segment
     struct Chunk { double a[4][2], b[4][2]; };
-    const auto request = [&](Chunk& k, int s, int half) {   // past the end: the last one once more
-        s = s < last ? s : last - 1;
-        const bool second = !PAIRED && s >= whole;
-        const int l0 = (second ? s - whole : s) * BK + half * KC;
+    const int chunks = 2 * last;                            // (a wavefront takes every fourth: two that share the lines of what lies along l at a time)
+    const auto request = [&](Chunk& k, int c) {             // past the end: the last one once more
+        c = c < chunks ? c : chunks - 1;
+        const bool second = !PAIRED && c >= 2 * whole;
+        const int l0 = (second ? c - 2 * whole : c) * KC;
         a.load(k.a, second ? a_shift : 0, g.lda, l0);
         b.load(k.b, second ? b_shift : 0, g.ldb, l0);
     };
@@ -181,17 +182,19 @@ __global__ __launch_bounds__(256, 2) void product_kernel(const Product<double> g
 #pragma unroll
                 for (int j = 0; j < 4; j++) acc[i][j] = Q::mma(k.a[i][s], k.b[j][s], acc[i][j]);
     };
-    if (first + wave < last) {
+    if (2 * first + wave < chunks) {
         Chunk one, two;
-        request(one, first + wave, 0);
-        for (int s = first + wave; s < last; s += 4) {
-            request(two, s, 1);
+        request(one, 2 * first + wave);
+        int c = 2 * first + wave;
+        for (; c + 4 < chunks; c += 8) {
+            request(two, c + 4);
             __builtin_amdgcn_sched_barrier(0);               // the requests go out before the products of the chunk that is here
             multiply(one);
-            request(one, s + 4, 0);
+            request(one, c + 8);
             __builtin_amdgcn_sched_barrier(0);
             multiply(two);
         }
+        if (c < chunks) multiply(one);
     }
     if (wave == 3 && g.inner % BK != 0 && last == all)
         for (int segment = 0; segment < g.segments; segment++)
