@@ -74,9 +74,12 @@ template <> struct Quad<double> {       // row 4 v + l / 16
 
 // The tile a block owns: consecutive block ids go round the 8 XCDs, each of which gets a contiguous run of tiles (bands of 8
 // tile rows, walked column by column), so that the blocks that share an L2 share operands.
+__device__ __forceinline__ unsigned place_of(unsigned block, unsigned blocks) {
+    const unsigned each = blocks / 8, rest = blocks % 8, xcd = block % 8, at = block / 8;
+    return xcd * each + (xcd < rest ? xcd : rest) + at;
+}
 __device__ __forceinline__ void own_tile(unsigned block, unsigned tiles, int tiles_m, int tiles_n, int& tm, int& tn) {
-    const unsigned each = tiles / 8, rest = tiles % 8, xcd = block % 8, at = block / 8;
-    const unsigned id = xcd * each + (xcd < rest ? xcd : rest) + at;
+    const unsigned id = place_of(block, tiles);
     const unsigned band = 8 * (unsigned)tiles_n, b = id / band, in = id - b * band;
     const unsigned height = (unsigned)tiles_m - b * 8 < 8 ? (unsigned)tiles_m - b * 8 : 8;
     tm = (int)(b * 8 + in % height);
@@ -749,17 +752,18 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
 
 // ---- few rows ----------------------------------------------------------------------------------------------------------
 // Up to 64 rows the weights' bytes bound the products, so they go from memory straight into the registers of the matrix
-// instructions (16 x 16 x 4, of the element type itself), each element once.  A wavefront owns 16 CW columns of both products and
+// instructions (16 x 16 x 4, of the element type itself), each element once.  A wavefront owns 16 columns of both products and
 // RT x 16 rows; the block's wavefronts share the contraction, U chunks of KC at a time in turn, and add their sums through LDS
 // in order.  Inside a chunk quarter q of a wavefront takes l from V q on, so that a lane's V values of A (and of weights stored
 // along l) are one 16-byte load.
 //
-// What the memory delivers depends on how the requests lie (4096 x 4096 twice in floats, 134 MB; reads alone): 64 bytes of a row per
-// wavefront and 256 blocks 32 us, 128 bytes and 256 blocks 25, 128 bytes and 128 blocks 34.  So a wavefront reads 128 bytes of a
-// row of weights, and where that leaves fewer blocks than units, g.parts blocks share a group of columns: each adds its sums
-// to memory, and the one that arrives last adds them all, part by part.  Weights stored along l are 128 bytes per column
-// (U chunks); there every group starts at another place of the contraction, because groups that walk in step
-// meet in the same memory channels (33 us in step, 28 apart).
+// What the memory delivers depends on how the requests lie.  A wavefront reads 64 bytes (f64 128) of a row of weights, half a line or, where
+// rows start inside one, parts of two: neighbouring columns belong to neighbouring blocks of one die, whose L2 then holds the other half
+// (8 rows x 4096 x 4096 in floats 26 us, 2048 x 3500 16; with blocks in launch order 32 and 25, with twice the columns per wavefront 26 and
+// 22).  Where the columns make fewer blocks than there are units, g.parts blocks share a group of columns: each adds its sums to
+// memory, and the one that arrives last adds them all, part by part.  Weights stored along l are 128 bytes per column (U chunks); there
+// every group starts at another place of the contraction, because groups that walk in step meet in the same memory channels (33 us in
+// step, 28 apart).
 //
 // The shared sums are written and read by atomic accesses of the whole device, which pass the caches of the eight dies one
 // by one; fences would write back and drop those caches whole (84 us instead of 27 for the call above).  What orders them: a wavefront
@@ -776,21 +780,20 @@ __device__ __forceinline__ Acc get_shared(const T* at) {
     for (int v = 0; v < 4; v++) x[v] = __hip_atomic_load(at + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return x;
 }
-template <typename T, int RT, int CW, bool ALONG, int EPI>
+template <typename T, int RT, bool ALONG, int EPI>
 __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int parts, T* partial, unsigned* arrived) {
     typedef Quad<T> Q;
     typedef typename Q::Acc Acc;
-    constexpr int WAVES = 8, V = 16 / sizeof(T), KC = 4 * V, U = 2, NA = EPI == GATED ? 1 : 2, FRAGMENTS = RT * CW;
+    constexpr int WAVES = 8, V = 16 / sizeof(T), KC = 4 * V, U = 2, NA = EPI == GATED ? 1 : 2;
     typedef T VecV __attribute__((ext_vector_type(V), aligned(sizeof(T))));
-    typedef T VecC __attribute__((ext_vector_type(CW), aligned(sizeof(T))));
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, c = lane & 15, q = lane >> 4;
-    const int part = blockIdx.x / (unsigned)g.tiles_n, group = blockIdx.x - (unsigned)part * (unsigned)g.tiles_n;
-    // the lane's CW neighbouring columns (moved back where they would pass the last one; what it shares with others it does not store)
-    const int own = group * 16 * CW + c * CW, n0 = own + CW <= g.cols ? own : g.cols - CW;
+    const unsigned place = place_of(blockIdx.x, gridDim.x);
+    const int part = place / (unsigned)g.tiles_n, group = place - (unsigned)part * (unsigned)g.tiles_n;
+    const int n = group * 16 + c, read = n < g.cols ? n : g.cols - 1;         // (past the end: the last column, not stored)
     const T *brow[2], *arow[NA][RT];
 #pragma unroll
-    for (int p = 0; p < 2; p++) brow[p] = g.B[p] + (int64_t)n0 * (ALONG ? g.ldb : 1);
+    for (int p = 0; p < 2; p++) brow[p] = g.B[p] + (int64_t)read * (ALONG ? g.ldb : 1);
 #pragma unroll
     for (int p = 0; p < NA; p++)
 #pragma unroll
@@ -798,26 +801,19 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int p
             const int m = r * 16 + c;
             arow[p][r] = g.A[p] + (int64_t)(m < g.rows ? m : g.rows - 1) * g.lda;
         }
-    Acc acc[2][RT][CW] = {};
-    struct Chunk { T a[NA][RT][V], b[2][CW][V]; };
+    Acc acc[2][RT] = {};
+    struct Chunk { T a[NA][RT][V], b[2][V]; };
     const auto load = [&](Chunk& k, int64_t l0) {            // a chunk that exists whole: no branch, so that the requests of several overlap
         const int64_t l = l0 + q * V;
 #pragma unroll
         for (int p = 0; p < 2; p++) {
             if constexpr (ALONG) {
+                const VecV w = *(const VecV*)(brow[p] + l);
 #pragma unroll
-                for (int j = 0; j < CW; j++) {
-                    const VecV w = *(const VecV*)(brow[p] + j * g.ldb + l);
-#pragma unroll
-                    for (int s = 0; s < V; s++) k.b[p][j][s] = w[s];
-                }
+                for (int s = 0; s < V; s++) k.b[p][s] = w[s];
             } else
 #pragma unroll
-                for (int s = 0; s < V; s++) {
-                    const VecC w = *(const VecC*)(brow[p] + (l + s) * g.ldb);
-#pragma unroll
-                    for (int j = 0; j < CW; j++) k.b[p][j][s] = w[j];
-                }
+                for (int s = 0; s < V; s++) k.b[p][s] = brow[p][(l + s) * g.ldb];
         }
 #pragma unroll
         for (int p = 0; p < NA; p++)
@@ -834,9 +830,7 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int p
         for (int s = 0; s < V; s++) {
             const bool in = l + s < g.inner;
 #pragma unroll
-            for (int p = 0; p < 2; p++)
-#pragma unroll
-                for (int j = 0; j < CW; j++) k.b[p][j][s] = in ? brow[p][ALONG ? j * g.ldb + l + s : (l + s) * g.ldb + j] : T(0);
+            for (int p = 0; p < 2; p++) k.b[p][s] = in ? brow[p][ALONG ? l + s : (l + s) * g.ldb] : T(0);
 #pragma unroll
             for (int p = 0; p < NA; p++)
 #pragma unroll
@@ -849,9 +843,7 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int p
 #pragma unroll
             for (int r = 0; r < RT; r++)
 #pragma unroll
-                for (int p = 0; p < 2; p++)
-#pragma unroll
-                    for (int j = 0; j < CW; j++) acc[p][r][j] = Q::mma(k.a[NA == 1 ? 0 : p][r][s], k.b[p][j][s], acc[p][r][j]);
+                for (int p = 0; p < 2; p++) acc[p][r] = Q::mma(k.a[NA == 1 ? 0 : p][r][s], k.b[p][s], acc[p][r]);
     };
     // The part's whole chunks, U at a time: wavefront w takes units w, w + WAVES, ...  What is left of the part, and the contraction's
     // last, partial chunk, belong to the last wavefront.
@@ -886,25 +878,23 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int p
         if (last == whole && part == parts - 1 && g.inner % KC != 0) { load_rest(one, (int64_t)whole * KC); multiply(one); }
     }
 
-    // the wavefronts' sums: [wave][product][row tile][column fragment][lane], a fragment's four values at a time
+    // the wavefronts' sums: [wave][product][row tile][lane], a fragment's four values at a time
     Acc* const sums = (Acc*)lds;
 #pragma unroll
     for (int p = 0; p < 2; p++)
 #pragma unroll
-        for (int r = 0; r < RT; r++)
-#pragma unroll
-            for (int j = 0; j < CW; j++) sums[((wave * 2 + p) * FRAGMENTS + r * CW + j) * 64 + lane] = acc[p][r][j];
+        for (int r = 0; r < RT; r++) sums[((wave * 2 + p) * RT + r) * 64 + lane] = acc[p][r];
     __syncthreads();
     const auto total = [&](int f, int p) {
-        Acc x = sums[(p * FRAGMENTS + f) * 64 + lane];
+        Acc x = sums[(p * RT + f) * 64 + lane];
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) x += sums[((w * 2 + p) * FRAGMENTS + f) * 64 + lane];
+        for (int w = 1; w < WAVES; w++) x += sums[((w * 2 + p) * RT + f) * 64 + lane];
         return x;
     };
-    T* const shared = partial + ((int64_t)group * (2 * FRAGMENTS * 64) + lane) * 4;          // part after part a whole result apart
-    const int64_t apart = (int64_t)g.tiles_n * (2 * FRAGMENTS * 64) * 4;
+    T* const shared = partial + ((int64_t)group * (2 * RT * 64) + lane) * 4;          // part after part a whole result apart
+    const int64_t apart = (int64_t)g.tiles_n * (2 * RT * 64) * 4;
     if (parts > 1) {
-        for (int f = wave; f < 2 * FRAGMENTS; f += WAVES) put_shared(shared + part * apart + f * 256, total(f % FRAGMENTS, f / FRAGMENTS));
+        for (int f = wave; f < 2 * RT; f += WAVES) put_shared(shared + part * apart + f * 256, total(f % RT, f / RT));
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wavefront's sums have arrived
         __syncthreads();
         unsigned* const order = (unsigned*)lds;
@@ -916,21 +906,20 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int p
         __syncthreads();
         if (*order != (unsigned)parts - 1) return;
     }
-    for (int f = wave; f < FRAGMENTS; f += WAVES) {
+    for (int f = wave; f < RT; f += WAVES) {
         Acc x, y;
         if (parts > 1) {
             x = get_shared<Acc>(shared + f * 256);
-            y = get_shared<Acc>(shared + (FRAGMENTS + f) * 256);
+            y = get_shared<Acc>(shared + (RT + f) * 256);
             for (int k = 1; k < parts; k++) {
                 x += get_shared<Acc>(shared + k * apart + f * 256);
-                y += get_shared<Acc>(shared + k * apart + (FRAGMENTS + f) * 256);
+                y += get_shared<Acc>(shared + k * apart + (RT + f) * 256);
             }
         } else { x = total(f, 0); y = total(f, 1); }
-        const int r = f / CW, n = n0 + f % CW;
-        if (n < own || n >= g.cols) continue;
+        if (n >= g.cols) continue;
 #pragma unroll
         for (int v = 0; v < 4; v++) {
-            const int m = r * 16 + Q::row(lane, v);
+            const int m = f * 16 + Q::row(lane, v);
             if (m >= g.rows) continue;
             const int64_t o = (int64_t)m * g.cols + n;
             if constexpr (EPI == GATED) {
@@ -1091,14 +1080,13 @@ static void launch_product(Device* dev, Product<T> g, const Split& s, bool a_alo
 }
 
 // The products of up to 64 rows: GATED, where both have the same A, or SUM, where each has its own.
-struct FewPlan { int row_tiles, width, groups, parts, steps_per_part; };
+struct FewPlan { int row_tiles, groups, parts, steps_per_part; };
 template <typename T>
-static FewPlan few_plan(const Device* dev, int64_t rows, int64_t cols, int64_t inner, bool along) {
+static FewPlan few_plan(const Device* dev, int64_t rows, int64_t cols, int64_t inner) {
     FewPlan f;
     const int64_t cus = dev->props.multiProcessorCount, chunk = 64 / (int64_t)sizeof(T), chunks = inner / chunk;
     f.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    f.width = sizeof(T) == 4 && !along && cols > 1 ? 2 : 1;              // 128 bytes of a row of weights
-    f.groups = (int)((cols + 16 * f.width - 1) / (16 * f.width));
+    f.groups = (int)((cols + 15) / 16);
     // one block per unit at least where the contraction is long enough: 16 chunks a part keep all wavefronts busy
     int64_t parts = f.groups >= cus ? 1 : (cus + f.groups - 1) / f.groups;
     if (parts > chunks / 16) parts = chunks / 16 > 0 ? chunks / 16 : 1;
@@ -1108,7 +1096,7 @@ static FewPlan few_plan(const Device* dev, int64_t rows, int64_t cols, int64_t i
     return f;
 }
 // the parts' sums, in elements: whole fragments of 16 x 16
-static uint64_t few_partial_elements(const FewPlan& f) { return f.parts > 1 ? (uint64_t)f.parts * f.groups * 2 * f.row_tiles * f.width * 256 : 0; }
+static uint64_t few_partial_elements(const FewPlan& f) { return f.parts > 1 ? (uint64_t)f.parts * f.groups * 2 * f.row_tiles * 256 : 0; }
 
 template <typename T, int EPI>
 static int launch_few(Device* dev, Product<T> g, const FewPlan& f, bool along, T* partial) {
@@ -1121,14 +1109,13 @@ static int launch_few(Device* dev, Product<T> g, const FewPlan& f, bool along, T
     hipError_t refused = hipSuccess;
     const auto go = [&](auto rt) {
         constexpr int RT = decltype(rt)::value;
-        const unsigned bytes = 8 * 2 * RT * f.width * 64 * 4 * sizeof(T);
+        const unsigned bytes = 8 * 2 * RT * 64 * 4 * sizeof(T);
         const auto run = [&](auto kernel) {
             if (bytes > 65536) refused = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
             if (refused == hipSuccess) hipLaunchKernelGGL(kernel, dim3((unsigned)(f.groups * f.parts)), dim3(512), bytes, dev->stream, g, f.parts, partial, arrived);
         };
-        if (along) run(few_rows_kernel<T, RT, 1, true, EPI>);
-        else if (f.width == 1) run(few_rows_kernel<T, RT, 1, false, EPI>);
-        else if constexpr (sizeof(T) == 4) run(few_rows_kernel<T, RT, 2, false, EPI>);
+        if (along) run(few_rows_kernel<T, RT, true, EPI>);
+        else run(few_rows_kernel<T, RT, false, EPI>);
     };
     if (f.row_tiles == 1)      go(std::integral_constant<int, 1>());
     else if (f.row_tiles == 2) go(std::integral_constant<int, 2>());
@@ -1167,7 +1154,7 @@ static int gated_forward(Device* dev, int fun, bool along, int64_t M, int64_t K,
     g.out[0] = H; g.out[1] = gate; g.out[2] = up;
     void* ws = nullptr;
     if (takes_few_rows<T>(M, K, N)) {
-        const FewPlan f = few_plan<T>(dev, M, N, K, along);
+        const FewPlan f = few_plan<T>(dev, M, N, K);
         if (const uint64_t need = few_partial_elements(f))
             if (int e = workspace(dev, need * sizeof(T), &ws)) return e;
         if (int e = launch_few<T, GATED>(dev, g, f, along, (T*)ws)) return e;
@@ -1199,7 +1186,7 @@ static int gated_backward(Device* dev, int fun, bool along, int64_t M, int64_t K
                           const T* E, T* dX, T* dWg, T* dWu) {
     const int64_t n = M * N;
     const Split sx = plan<T>(dev, false, M, K, N, 2), sw = plan<T>(dev, true, K, N, M, 1);
-    const FewPlan few = few_plan<T>(dev, M, K, N, !along);
+    const FewPlan few = few_plan<T>(dev, M, K, N);
     const bool is_few = takes_few_rows<T>(M, K, N);
     const uint64_t px = dX ? is_few ? few_partial_elements(few) : partial_elements(sx, false, M, K) : 0, pw = dWg ? partial_elements(sw, true, K, N) : 0;
     const bool two_x = dX && !is_few && two_planes<T>(M, K, 2 * N), two_w = dWg && two_planes<T>(K, 2 * N, M);
