@@ -8,9 +8,9 @@
 // (forward, weight gradients) are PAIRED: a tile holds the same columns of both, half each, so that A is staged once for both and
 // f(gate) up is formed in the registers that hold the sums.  dX is one product over a contraction of two segments, (dg, Wg) and then
 // (du, Wu).  What bounds them and what runs:
-//   few_rows_kernel        up to 32 rows (64 with few weights or in f64): the weights' bytes; straight from memory into registers
+//   few_rows_kernel        up to 32 rows (64 with few weights): the weights' bytes; straight from memory into registers
 //   split_product_kernel   f32: the 16-bit matrix cores, which take floats as sums of 16-bit numbers; tiles through LDS
-//   product_kernel         f64: the f64 matrix cores; tiles through LDS
+//   product_kernel         f64: the f64 matrix cores; straight from memory into registers
 //   product_join_kernel    adds parts of the contraction where tiles alone would not fill the chip
 //   gated_errors_kernel    dg and du, once, for the three products of the backward pass
 #include "nk_internal.h"
@@ -86,10 +86,12 @@ __device__ __forceinline__ void own_tile(unsigned block, unsigned tiles, int til
     tn = (int)(in / height);
 }
 
-// The f64 products: tiles of 64 x 64, the contraction shared by the block's 4 wavefronts, steps of 16 l in turn.  Every wavefront holds the
+// The f64 products: tiles of 64 x 64, the contraction shared by the block's 4 wavefronts, chunks of 8 l in turn.  Every wavefront holds the
 // whole tile (4 x 4 fragments of 16 x 16) and nothing it reads is another's, so its operands go from memory straight into the
 // registers of the matrix instructions: 32 instructions of 64 cycles to a chunk of 8 l, whose eight 16-byte loads went out a chunk
 // before.  No barrier until the sums meet in LDS, where each wavefront takes a quarter of the tile.
+// 2048^3 forward 59 TFLOP/s, 512 x 512 x 2048 50 (tiles staged in LDS for 4 wavefronts of 32 x 32: 52 and 41): there the matrix cores are
+// busy three quarters of the time that a unit has work, the rest is the first requests, the sums and f.
 //
 // Quarter q of a wavefront takes l = 2 q, 2 q + 1 of a chunk.  Operands that lie along l: a lane's two values are one load.  Operands that
 // lie across: a lane loads two neighbouring rows (columns) of one l, so fragments 2 h and 2 h + 1 hold rows 32 h + 2 r and 32 h + 2 r + 1.
@@ -752,18 +754,22 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
 
 // ---- few rows ----------------------------------------------------------------------------------------------------------
 // Up to 64 rows the weights' bytes bound the products, so they go from memory straight into the registers of the matrix
-// instructions (16 x 16 x 4, of the element type itself), each element once.  A wavefront owns 16 columns of both products and
+// instructions (16 x 16 x 4, of the element type itself), each element once.  A wavefront owns 16 CW columns of both products and
 // RT x 16 rows; the block's wavefronts share the contraction, U chunks of KC at a time in turn, and add their sums through LDS
 // in order.  Inside a chunk quarter q of a wavefront takes l from V q on, so that a lane's V values of A (and of weights stored
 // along l) are one 16-byte load.
 //
-// What the memory delivers depends on how the requests lie.  A wavefront reads 64 bytes (f64 128) of a row of weights, half a line or, where
-// rows start inside one, parts of two: neighbouring columns belong to neighbouring blocks of one die, whose L2 then holds the other half
-// (8 rows x 4096 x 4096 in floats 26 us, 2048 x 3500 16; with blocks in launch order 32 and 25, with twice the columns per wavefront 26 and
-// 22).  Where the columns make fewer blocks than there are units, g.parts blocks share a group of columns: each adds its sums to
-// memory, and the one that arrives last adds them all, part by part.  Weights stored along l are 128 bytes per column (U chunks); there
-// every group starts at another place of the contraction, because groups that walk in step meet in the same memory channels (33 us in
-// step, 28 apart).
+// What the memory delivers depends on how the requests lie (weights that no cache holds):
+//  - Weights by row, in floats: one row tile reads 128 bytes of a row per wavefront (CW 2; 1 x 4096 x 4096 28 us, 64 bytes 34).  Two row
+//    tiles and more read 64 and one chunk at a time (32 x 2048 x 3500 28 us, 128 bytes 35), four because the rest does not fit their registers.
+//  - Weights stored along l: 128 bytes per column (U 2; 16 x 4096 x 4096 26 us, U 1 31); four row tiles take one chunk (64 x 2048 x
+//    2048 19 us, U 2 24).  There every group starts at another place of the contraction, because groups that walk in step meet in the
+//    same memory channels (33 us in step, 28 apart).
+//  - Neighbouring columns belong to neighbouring blocks of one die, whose L2 holds the lines that they share where rows do not start with
+//    a line (16 x 3001 x 1301 22 -> 18 us).
+//  - Where the columns make fewer blocks than there are units, g.parts blocks share a group of columns: each adds its sums to memory,
+//    and the one that arrives last adds them all, part by part.  As many parts as units hold at once, since a unit with two blocks
+//    would end last (1 x 2048 x 3500, 110 groups: 2 parts 16 us, 3 parts 23).
 //
 // The shared sums are written and read by atomic accesses of the whole device, which pass the caches of the eight dies one
 // by one; fences would write back and drop those caches whole (84 us instead of 27 for the call above).  What orders them: a wavefront
@@ -780,20 +786,22 @@ __device__ __forceinline__ Acc get_shared(const T* at) {
     for (int v = 0; v < 4; v++) x[v] = __hip_atomic_load(at + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return x;
 }
-template <typename T, int RT, bool ALONG, int EPI>
+template <typename T, int RT, int CW, bool ALONG, int EPI>
 __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int parts, T* partial, unsigned* arrived) {
     typedef Quad<T> Q;
     typedef typename Q::Acc Acc;
-    constexpr int WAVES = 8, V = 16 / sizeof(T), KC = 4 * V, U = 2, NA = EPI == GATED ? 1 : 2;
+    constexpr int WAVES = 8, V = 16 / sizeof(T), KC = 4 * V, U = RT <= 2 && (ALONG || CW == 2) ? 2 : 1, NA = EPI == GATED ? 1 : 2, FRAGMENTS = RT * CW;
     typedef T VecV __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+    typedef T VecC __attribute__((ext_vector_type(CW), aligned(sizeof(T))));
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, c = lane & 15, q = lane >> 4;
     const unsigned place = place_of(blockIdx.x, gridDim.x);
     const int part = place / (unsigned)g.tiles_n, group = place - (unsigned)part * (unsigned)g.tiles_n;
-    const int n = group * 16 + c, read = n < g.cols ? n : g.cols - 1;         // (past the end: the last column, not stored)
+    // the lane's CW neighbouring columns (moved back where they would pass the last one; what it shares with others it does not store)
+    const int own = group * 16 * CW + c * CW, n0 = own + CW <= g.cols ? own : g.cols - CW;
     const T *brow[2], *arow[NA][RT];
 #pragma unroll
-    for (int p = 0; p < 2; p++) brow[p] = g.B[p] + (int64_t)read * (ALONG ? g.ldb : 1);
+    for (int p = 0; p < 2; p++) brow[p] = g.B[p] + (int64_t)n0 * (ALONG ? g.ldb : 1);
 #pragma unroll
     for (int p = 0; p < NA; p++)
 #pragma unroll
@@ -801,19 +809,26 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int p
             const int m = r * 16 + c;
             arow[p][r] = g.A[p] + (int64_t)(m < g.rows ? m : g.rows - 1) * g.lda;
         }
-    Acc acc[2][RT] = {};
-    struct Chunk { T a[NA][RT][V], b[2][V]; };
+    Acc acc[2][RT][CW] = {};
+    struct Chunk { T a[NA][RT][V], b[2][CW][V]; };
     const auto load = [&](Chunk& k, int64_t l0) {            // a chunk that exists whole: no branch, so that the requests of several overlap
         const int64_t l = l0 + q * V;
 #pragma unroll
         for (int p = 0; p < 2; p++) {
             if constexpr (ALONG) {
-                const VecV w = *(const VecV*)(brow[p] + l);
 #pragma unroll
-                for (int s = 0; s < V; s++) k.b[p][s] = w[s];
+                for (int j = 0; j < CW; j++) {
+                    const VecV w = *(const VecV*)(brow[p] + j * g.ldb + l);
+#pragma unroll
+                    for (int s = 0; s < V; s++) k.b[p][j][s] = w[s];
+                }
             } else
 #pragma unroll
-                for (int s = 0; s < V; s++) k.b[p][s] = brow[p][(l + s) * g.ldb];
+                for (int s = 0; s < V; s++) {
+                    const VecC w = *(const VecC*)(brow[p] + (l + s) * g.ldb);
+#pragma unroll
+                    for (int j = 0; j < CW; j++) k.b[p][j][s] = w[j];
+                }
         }
 #pragma unroll
         for (int p = 0; p < NA; p++)
@@ -830,7 +845,9 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int p
         for (int s = 0; s < V; s++) {
             const bool in = l + s < g.inner;
 #pragma unroll
-            for (int p = 0; p < 2; p++) k.b[p][s] = in ? brow[p][ALONG ? l + s : (l + s) * g.ldb] : T(0);
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int j = 0; j < CW; j++) k.b[p][j][s] = in ? brow[p][ALONG ? j * g.ldb + l + s : (l + s) * g.ldb + j] : T(0);
 #pragma unroll
             for (int p = 0; p < NA; p++)
 #pragma unroll
@@ -843,7 +860,9 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int p
 #pragma unroll
             for (int r = 0; r < RT; r++)
 #pragma unroll
-                for (int p = 0; p < 2; p++) acc[p][r] = Q::mma(k.a[NA == 1 ? 0 : p][r][s], k.b[p][s], acc[p][r]);
+                for (int p = 0; p < 2; p++)
+#pragma unroll
+                    for (int j = 0; j < CW; j++) acc[p][r][j] = Q::mma(k.a[NA == 1 ? 0 : p][r][s], k.b[p][j][s], acc[p][r][j]);
     };
     // The part's whole chunks, U at a time: wavefront w takes units w, w + WAVES, ...  What is left of the part, and the contraction's
     // last, partial chunk, belong to the last wavefront.
@@ -878,23 +897,25 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int p
         if (last == whole && part == parts - 1 && g.inner % KC != 0) { load_rest(one, (int64_t)whole * KC); multiply(one); }
     }
 
-    // the wavefronts' sums: [wave][product][row tile][lane], a fragment's four values at a time
+    // the wavefronts' sums: [wave][product][row tile][column fragment][lane], a fragment's four values at a time
     Acc* const sums = (Acc*)lds;
 #pragma unroll
     for (int p = 0; p < 2; p++)
 #pragma unroll
-        for (int r = 0; r < RT; r++) sums[((wave * 2 + p) * RT + r) * 64 + lane] = acc[p][r];
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int j = 0; j < CW; j++) sums[((wave * 2 + p) * FRAGMENTS + r * CW + j) * 64 + lane] = acc[p][r][j];
     __syncthreads();
     const auto total = [&](int f, int p) {
-        Acc x = sums[(p * RT + f) * 64 + lane];
+        Acc x = sums[(p * FRAGMENTS + f) * 64 + lane];
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) x += sums[((w * 2 + p) * RT + f) * 64 + lane];
+        for (int w = 1; w < WAVES; w++) x += sums[((w * 2 + p) * FRAGMENTS + f) * 64 + lane];
         return x;
     };
-    T* const shared = partial + ((int64_t)group * (2 * RT * 64) + lane) * 4;          // part after part a whole result apart
-    const int64_t apart = (int64_t)g.tiles_n * (2 * RT * 64) * 4;
+    T* const shared = partial + ((int64_t)group * (2 * FRAGMENTS * 64) + lane) * 4;          // part after part a whole result apart
+    const int64_t apart = (int64_t)g.tiles_n * (2 * FRAGMENTS * 64) * 4;
     if (parts > 1) {
-        for (int f = wave; f < 2 * RT; f += WAVES) put_shared(shared + part * apart + f * 256, total(f % RT, f / RT));
+        for (int f = wave; f < 2 * FRAGMENTS; f += WAVES) put_shared(shared + part * apart + f * 256, total(f % FRAGMENTS, f / FRAGMENTS));
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wavefront's sums have arrived
         __syncthreads();
         unsigned* const order = (unsigned*)lds;
@@ -906,20 +927,21 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const Product<T> g, int p
         __syncthreads();
         if (*order != (unsigned)parts - 1) return;
     }
-    for (int f = wave; f < RT; f += WAVES) {
+    for (int f = wave; f < FRAGMENTS; f += WAVES) {
         Acc x, y;
         if (parts > 1) {
             x = get_shared<Acc>(shared + f * 256);
-            y = get_shared<Acc>(shared + (RT + f) * 256);
+            y = get_shared<Acc>(shared + (FRAGMENTS + f) * 256);
             for (int k = 1; k < parts; k++) {
                 x += get_shared<Acc>(shared + k * apart + f * 256);
-                y += get_shared<Acc>(shared + k * apart + (RT + f) * 256);
+                y += get_shared<Acc>(shared + k * apart + (FRAGMENTS + f) * 256);
             }
         } else { x = total(f, 0); y = total(f, 1); }
-        if (n >= g.cols) continue;
+        const int r = f / CW, n = n0 + f % CW;
+        if (n < own || n >= g.cols) continue;
 #pragma unroll
         for (int v = 0; v < 4; v++) {
-            const int m = f * 16 + Q::row(lane, v);
+            const int m = r * 16 + Q::row(lane, v);
             if (m >= g.rows) continue;
             const int64_t o = (int64_t)m * g.cols + n;
             if constexpr (EPI == GATED) {
@@ -1080,23 +1102,27 @@ static void launch_product(Device* dev, Product<T> g, const Split& s, bool a_alo
 }
 
 // The products of up to 64 rows: GATED, where both have the same A, or SUM, where each has its own.
-struct FewPlan { int row_tiles, groups, parts, steps_per_part; };
+struct FewPlan { int row_tiles, width, groups, parts, steps_per_part; };
 template <typename T>
-static FewPlan few_plan(const Device* dev, int64_t rows, int64_t cols, int64_t inner) {
+static FewPlan few_plan(const Device* dev, int64_t rows, int64_t cols, int64_t inner, bool along) {
     FewPlan f;
     const int64_t cus = dev->props.multiProcessorCount, chunk = 64 / (int64_t)sizeof(T), chunks = inner / chunk;
     f.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    f.groups = (int)((cols + 15) / 16);
-    // one block per unit at least where the contraction is long enough: 16 chunks a part keep all wavefronts busy
-    int64_t parts = f.groups >= cus ? 1 : (cus + f.groups - 1) / f.groups;
-    if (parts > chunks / 16) parts = chunks / 16 > 0 ? chunks / 16 : 1;
+    f.width = sizeof(T) == 4 && f.row_tiles == 1 && !along && cols > 1 ? 2 : 1;
+    f.groups = (int)((cols + 16 * f.width - 1) / (16 * f.width));
+    // So many parts that the unit with the most blocks has the least to do (a hundredth of the whole charged for joining each), of at least
+    // 16 chunks, which keep all wavefronts busy.
+    int64_t parts = 1;
+    const auto busiest = [&](int64_t p) { return (double)((f.groups * p + cus - 1) / cus) / p + 0.01 * p; };
+    for (int64_t p = 2; p <= 16 && p <= chunks / 16 && f.groups < cus; p++)
+        if (busiest(p) < busiest(parts)) parts = p;
     f.steps_per_part = chunks ? (int)((chunks + parts - 1) / parts) : 1;
     f.steps_per_part += f.steps_per_part & 1;                            // (chunks are taken in twos)
     f.parts = chunks ? (int)((chunks + f.steps_per_part - 1) / f.steps_per_part) : 1;
     return f;
 }
 // the parts' sums, in elements: whole fragments of 16 x 16
-static uint64_t few_partial_elements(const FewPlan& f) { return f.parts > 1 ? (uint64_t)f.parts * f.groups * 2 * f.row_tiles * 256 : 0; }
+static uint64_t few_partial_elements(const FewPlan& f) { return f.parts > 1 ? (uint64_t)f.parts * f.groups * 2 * f.row_tiles * f.width * 256 : 0; }
 
 template <typename T, int EPI>
 static int launch_few(Device* dev, Product<T> g, const FewPlan& f, bool along, T* partial) {
@@ -1109,13 +1135,14 @@ static int launch_few(Device* dev, Product<T> g, const FewPlan& f, bool along, T
     hipError_t refused = hipSuccess;
     const auto go = [&](auto rt) {
         constexpr int RT = decltype(rt)::value;
-        const unsigned bytes = 8 * 2 * RT * 64 * 4 * sizeof(T);
+        const unsigned bytes = 8 * 2 * RT * f.width * 64 * 4 * sizeof(T);
         const auto run = [&](auto kernel) {
             if (bytes > 65536) refused = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
             if (refused == hipSuccess) hipLaunchKernelGGL(kernel, dim3((unsigned)(f.groups * f.parts)), dim3(512), bytes, dev->stream, g, f.parts, partial, arrived);
         };
-        if (along) run(few_rows_kernel<T, RT, true, EPI>);
-        else run(few_rows_kernel<T, RT, false, EPI>);
+        if (along) run(few_rows_kernel<T, RT, 1, true, EPI>);
+        else if (f.width == 1) run(few_rows_kernel<T, RT, 1, false, EPI>);
+        else if constexpr (sizeof(T) == 4 && RT == 1) run(few_rows_kernel<T, RT, 2, false, EPI>);
     };
     if (f.row_tiles == 1)      go(std::integral_constant<int, 1>());
     else if (f.row_tiles == 2) go(std::integral_constant<int, 2>());
@@ -1131,11 +1158,12 @@ template <typename T> static bool two_planes(int64_t rows, int64_t cols, int64_t
     const double saved_us = 6.0 * rows * cols * inner / 1.1e9, cost_us = 6.0 + 4.0 * (rows + cols) * inner / 4.5e6;
     return sizeof(T) == 4 && saved_us > cost_us;
 }
-// Whether M rows go to few_rows_kernel.  Above 32 rows it holds four row tiles per wavefront and is bound by the matrix instructions: in
-// f32, whose tiles run on the faster 16-bit ones, only while the weights are few (64 rows forward, microseconds, few rows / tiles:
-// 1024 x 1024 17 / 20, 300 x 2000 13 / 20, 4096 x 4096 83 / 63; f64 18 / 24, 14 / 17, 109 / 188).
+// Whether M rows go to few_rows_kernel.  Above 32 rows it holds four row tiles per wavefront and is bound by its matrix instructions, of
+// which the tiles have faster ones (f32) or feed them better (f64): there only while the weights are few, where the tiles' slices are too
+// short to fill the chip.  64 rows, weights by row, few rows / tiles in microseconds, forward and d_X: f32 1024 x 1024 (8 MB) 12 / 19 and
+// 16 / 23, 2000 x 1500 (24 MB) 33 / 23 and 32 / 29; f64 700 x 150 (2 MB) 12 / 13 and 11 / 17, 300 x 2000 (10 MB) 14 / 16 and 34 / 23.
 template <typename T> static bool takes_few_rows(int64_t M, int64_t K, int64_t N) {
-    return M <= 32 || (M <= 64 && (sizeof(T) == 8 || 2 * K * N * (int64_t)sizeof(T) < 48000000));
+    return M <= 32 || (M <= 64 && 2 * K * N * (int64_t)sizeof(T) < (sizeof(T) == 8 ? 5000000 : 20000000));
 }
 static void add_job(ScaleJobs& jobs, const float* p, const float* second, int64_t ld, int64_t count, int64_t length, bool along, int* out) {
     jobs.job[jobs.n++] = {{p, second}, ld, (int)count, (int)length, along, out, (unsigned)(along ? (count + 7) / 8 : (count + 31) / 32)};
@@ -1154,7 +1182,7 @@ static int gated_forward(Device* dev, int fun, bool along, int64_t M, int64_t K,
     g.out[0] = H; g.out[1] = gate; g.out[2] = up;
     void* ws = nullptr;
     if (takes_few_rows<T>(M, K, N)) {
-        const FewPlan f = few_plan<T>(dev, M, N, K);
+        const FewPlan f = few_plan<T>(dev, M, N, K, along);
         if (const uint64_t need = few_partial_elements(f))
             if (int e = workspace(dev, need * sizeof(T), &ws)) return e;
         if (int e = launch_few<T, GATED>(dev, g, f, along, (T*)ws)) return e;
@@ -1186,7 +1214,7 @@ static int gated_backward(Device* dev, int fun, bool along, int64_t M, int64_t K
                           const T* E, T* dX, T* dWg, T* dWu) {
     const int64_t n = M * N;
     const Split sx = plan<T>(dev, false, M, K, N, 2), sw = plan<T>(dev, true, K, N, M, 1);
-    const FewPlan few = few_plan<T>(dev, M, K, N);
+    const FewPlan few = few_plan<T>(dev, M, K, N, !along);
     const bool is_few = takes_few_rows<T>(M, K, N);
     const uint64_t px = dX ? is_few ? few_partial_elements(few) : partial_elements(sx, false, M, K) : 0, pw = dWg ? partial_elements(sw, true, K, N) : 0;
     const bool two_x = dX && !is_few && two_planes<T>(M, K, 2 * N), two_w = dWg && two_planes<T>(K, 2 * N, M);
