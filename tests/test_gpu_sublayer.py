@@ -664,3 +664,19 @@ def test_axes_beyond_a_launch_are_refused(device):
             assert b"2^27" in lib.nk_last_error()
     assert lib.nk_layer_norm(h, 0, 1, (1 << 27) - 1023, p, 1 << 27, p, p, 1e-5, p, 0, 0) != 0
     assert b"2^27" in lib.nk_last_error()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("along", [False, True])
+@pytest.mark.parametrize("M,K,N", [(100, 1, 1), (100, 1, 40), (100, 40, 1), (5, 1, 40), (5, 40, 1), (70, 2, 3), (130, 3, 2), (80, 65, 33), (80, 33, 65)])
+def test_gated_products_with_thin_axes_are_exact(device, dt, along, M, K, N):
+    """Axes of one to three elements and one past a tile, where columns are read by twos."""
+    test_gated_products_of_small_integers_are_exact(device, dt, along, M, K, N)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("along", [False, True])
+@pytest.mark.parametrize("M,K,N", [(1, 3001, 1301), (20, 3001, 1301), (40, 500, 701), (64, 1501, 700), (33, 1700, 1600)])
+def test_gated_few_rows_in_parts_and_on_tiles(device, dt, along, M, K, N):
+    """Parts that do not divide the contraction, and both sides of the choice between few rows and tiles."""
+    check_gated(device, dt, "gelu", M, K, N, along)
