@@ -282,14 +282,14 @@ int nk_dropout(nk_dev dev, int dtype, int rank, nk_buf drn, const int32_t* drn_c
  * stored as [N,K]; everything else is row-major.  gate and up ([M,N], both or neither 0) are written for the backward pass.
  * f64 products run on the f64 matrix cores, f32 products of up to 32 rows (64 where the weights are small) on those of f32.  Larger
  * f32 products take the 16-bit matrix cores in one of two ways, whichever is estimated to be faster, and add in f32:
- *   - operands as sums of three bfloat16 numbers (24 bits, exactly the operand's where its magnitude is 2^-110 or more), every product
- *     as its six partial products above 2^-24 of it;
- *   - operands as sums of two half-precision numbers after a power of two per row of X and per column of a weight: 2^-16 of the largest
- *     magnitude of that row or column or more keeps 22 bits and a sign, smaller numbers are off by at most 2^-40 of the largest.
- *     Rows and columns below an outlier or spread over more than 24 binades, and any with an infinity or NaN, are found beforehand
- *     and take the first way.
- * The error stays within 1e-5 of sum_k (|x_ik| + 2^-23 X_i) (|w_kj| + 2^-23 W_j), X_i and W_j the largest magnitudes of row i of X
- * and column j of W (the first way: within 1e-5 of sum_k |x_ik| |w_kj|, like nk_matmul); infinities, NaN and overflow give what f32
+ *   - operands as sums of three bfloat16 numbers: 24 bits, exactly the operand's where its magnitude is 2^-110 or more (off by up to 2^-134 below),
+ *     every product as its six largest partial products, the others at most 2^-25 of it each;
+ *   - operands as sums of two half-precision numbers after a power of two per row of X and per column of a weight (in d_X one for both errors
+ *     and one for both weights): what is 2^-16 of the largest magnitude of that row or column or more is held to 2^-23, what is 2^-20 of it to 2^-19.
+ *     Smaller numbers are counted.  A result so small that those of its row and column could matter to it is computed again from the floats;
+ *     rows and columns of which more than two and a 256th are that small, and any with an infinity or NaN, take the first way.
+ * Either way, those 2^-134 apart, the operands' part of the error stays within 2^-17 of sum_k |x_ik| |w_kj|, whatever meets what (on average it is
+ * below the roundings of a product of floats); the roundings of the f32 sums come on top, as in any such product.  Infinities, NaN and overflow give what f32
  * arithmetic gives.  Every sum is added in an order that shape, layout and alignment fix.  M, K, N <= 2^27 - 1024. */
 int nk_gated_matmul(nk_dev dev, int fun_id, int dtype, int weight_layout, int64_t M, int64_t K, int64_t N, nk_buf X, nk_buf Wg, nk_buf Wu,
                     nk_buf drn, nk_buf gate, nk_buf up);

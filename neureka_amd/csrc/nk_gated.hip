@@ -260,20 +260,29 @@ __global__ __launch_bounds__(256, 2) void product_kernel(const Product<double> g
 //
 // 3: bfloat16, any operands.  A float is the sum of three, each the rest of the ones before rounded to nearest: 3 x 8 bits hold its 24
 // (below 2^-110 the last leaves bfloat16's range: off by at most 2^-134).  The six largest of the nine partial products are added,
-// x0 y0, x0 y1, x1 y0, x1 y1, x0 y2, x2 y0; the rest is at most 2^-26 of x y each.  A non-finite operand has no such sum
+// x0 y0, x0 y1, x1 y0, x1 y1, x0 y2, x2 y0; the rest is at most 2^-25 of x y each.  A non-finite operand has no such sum
 // (infinity - infinity), so a wavefront that finds a non-finite result computes that fragment of its tile once more with the f32
 // instruction, straight from memory: what comes out is what f32 arithmetic gives.
 //
 // 2: half precision, half as many partial products: x0 y0, x0 y1, x1 y0.  Two halves hold a float to 2^-23 of it (2^-25 on average)
 // and x1 y1 is at most 2^-22 of x y (2^-25 on average, of either sign), as long as they stay within the type's few binades.
-// So a launch before finds, for every row of A and of B, the power of two that brings its largest magnitude below
-// 2^15; what is 2^-16 of that or more keeps all its bits, and smaller numbers are off by at most 2^-40 of the largest.
-// A row where that could show is marked, and tiles with a marked row take three planes: one with an infinity or NaN, or where in more
-// than a quarter of those of its 64 stretches that are not all zero either everything is below 2^-16 of the largest or something other
-// than zero below 2^-24.  The first is an outlier above the row, the second a spread that the other operand may undo (columns of X scaled
-// one way, rows of a weight the other), where a small number counts as much as a large one.  Normally distributed numbers
-// have one element in 10^6 below 2^-24 of the largest, so rows of them are not marked.
-constexpr int MARKED = 1 << 30;                              // in place of a row's exponent
+// So a launch before finds, for every row of A and of B, the power of two that brings its largest magnitude to [2^14, 2^15).  The planes
+// end at multiples of 2^-24, so a number is off by at most 2^-25 there: 2^-19 of itself or less from 2^-6 on, too much below.
+// What such SMALL numbers are worth depends on what they meet (zeros may stand where their row is large), so no property of a row
+// alone can tell.  The launch counts them, and each result is judged by what it came to: with a and b small numbers in its row and its column,
+// each of which meets less than 2^15, it is off by less than (a + b) 2^-10 (1 + 2^-9), so one of UNCERTAIN (a + b) or more is right to 2^-18.
+// A result below that is computed again from the floats.  In all, an error of at most 2^-17 of the sum of |x y|, with whatever rows meet; on
+// average the planes' 2^-25.  Rows of which more than two and a 256th are small, where many results would have to be computed again, and
+// rows with an infinity or NaN are marked, and a tile with a marked row takes three planes.  Of rows of 4096 normally distributed numbers one in 130
+// has a small one, and one result in 10^9 is computed again; rows of dg (products of two such numbers and a slope) have one or two, eight at most.
+constexpr int MARKED = 1 << 30, EMPTY = 1 << 29;             // notes on a row: three planes; nothing but zeros; else how many are small, and the exponent
+constexpr int MOST_SMALL = (1 << 20) - 1;
+constexpr float UNCERTAIN = 260.0f;                          // 2^-10 (1 + 2^-9) / 2^-18, rounded up
+__device__ __forceinline__ int note_of(int exponent, int small) { return small << 9 | (exponent + 256); }
+__device__ __forceinline__ int exponent_of(int note) { return (note & 511) - 256; }
+__device__ __forceinline__ int small_of(int note) { return note >> 9 & MOST_SMALL; }
+// the least magnitude, in the planes' scale, of a result that is certain; a row of zeros has results of zero whatever it meets
+__device__ __forceinline__ float least_certain(int a, int b) { return (a | b) & EMPTY ? 0.0f : UNCERTAIN * (float)(small_of(a) + small_of(b)); }
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -317,27 +326,40 @@ template <> struct Partial<2> {
     }
 };
 
-// The exponents of up to five operands' rows (`count` rows of `length`, together with those of a second matrix where there is
+// The notes on up to five operands' rows (`count` rows of `length`, together with those of a second matrix where there is
 // one), blocks dealt out operand by operand.  Rows that lie along memory: a wavefront each, 64 stretches of every 64th 4 elements.
-// Rows across memory: 32 of them per block, 64 stretches of every 64th element.  Bound by memory: three operands of 4096 x 4096 in
-// 50 us, 4.0 TB/s.
+// Rows across memory: 32 of them per block, 64 stretches of every 64th element.  A stretch whose third least number is
+// small for its row is read again to count.  Bound by memory: three operands of 4096 x 4096 in 53-60 us, 3.3-3.8 TB/s.
 struct ScaleJob { const float* p[2]; int64_t ld; int count, length; bool along; int* out; unsigned blocks; };
 struct ScaleJobs { ScaleJob job[5]; int n; };
+__device__ __forceinline__ unsigned magnitude(float x) { return __builtin_bit_cast(unsigned, x) & 0x7fffffffu; }
 struct Range {                                               // of the magnitudes of a stretch, as their bits
-    unsigned most = 0, below_least = ~0u;                   // the least other than zero, less one
+    unsigned most = 0, least[3] = {~0u, ~0u, ~0u};          // the least other than zero, less one, in order
     __device__ __forceinline__ void add(float x) {
-        const unsigned u = __builtin_bit_cast(unsigned, x) & 0x7fffffffu;
+        const unsigned u = magnitude(x);
         most = u > most ? u : most;
-        below_least = u - 1 < below_least ? u - 1 : below_least;
+        unsigned w = u - 1;
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            const unsigned above = w > least[k] ? w : least[k];
+            least[k] = w < least[k] ? w : least[k];
+            w = above;
+        }
     }
-    __device__ __forceinline__ bool far_below(unsigned largest) const {
-        return most != 0 && ((most >> 23) + 16 < (largest >> 23) || (below_least >> 23) + 24 < (largest >> 23));
-    }
+    // how many are small, where the third is not
+    __device__ __forceinline__ unsigned below(unsigned bound) const { return (least[0] < bound) + (least[1] < bound); }
 };
-__device__ __forceinline__ int exponent_for(unsigned largest, int low, int some) {      // low of some stretches that are not all zero are far below the largest
-    if (largest >= 0x7f800000u || 4 * low > some) return MARKED;
+// A magnitude other than zero is small in its row if, less one, it is below this: below 2^-6 times 2^14 over the largest's power of two.  (A largest
+// number below 2^-111 is brought up by 2^126 alone: then even the least of the floats are multiples of 2^-23 there, and exact.)
+__device__ __forceinline__ unsigned small_bound(unsigned largest) {
+    const unsigned e = largest >> 23;
+    return (e <= 15 || e >= 255 ? 1u : e <= 20 ? 1u << (e + 2) : (e - 20) << 23) - 1;
+}
+__device__ __forceinline__ int note_on(unsigned largest, unsigned small, int64_t elements) {
+    const int64_t most = 2 + elements / 256;
+    if (largest >= 0x7f800000u || small > (most < MOST_SMALL ? most : MOST_SMALL)) return MARKED;
     const int e = 14 + 127 - (int)(largest >> 23);
-    return largest == 0 ? 0 : e < 126 ? e : 126;
+    return largest == 0 ? EMPTY | note_of(0, 0) : note_of(e < 126 ? e : 126, (int)small);
 }
 
 __global__ __launch_bounds__(512) void operand_scales_kernel(const ScaleJobs jobs) {
@@ -345,50 +367,79 @@ __global__ __launch_bounds__(512) void operand_scales_kernel(const ScaleJobs job
     int which = 0;
     while (which + 1 < jobs.n && block >= jobs.job[which].blocks) block -= jobs.job[which++].blocks;
     const ScaleJob j = jobs.job[which];
+    const int64_t elements = (int64_t)j.length * (j.p[1] ? 2 : 1);
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     if (j.along) {
         const int row = (int)block * 8 + wave;
         if (row >= j.count) return;
-        Range m;
-        for (int k = 0; k < 2; k++) {
-            if (!j.p[k]) continue;
-            const float* const at = j.p[k] + (int64_t)row * j.ld;
-            int i = lane * 4;
-#pragma unroll 4
-            for (; i + 4 <= j.length; i += 256) {
-                const f32x4 v = *(const f32x4_any*)(at + i);
+        const auto visit = [&](auto take) {                  // the lane's stretch, of both matrices
+            for (int k = 0; k < 2; k++) {
+                if (!j.p[k]) continue;
+                const float* const at = j.p[k] + (int64_t)row * j.ld;
+                int i = lane * 4;
+                for (; i + 3 * 256 + 4 <= j.length; i += 4 * 256) {          // four requests on their way
+                    f32x4 v[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) m.add(v[e]);
+                    for (int u = 0; u < 4; u++) v[u] = *(const f32x4_any*)(at + i + u * 256);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) take(v[u][e]);
+                }
+                for (; i + 4 <= j.length; i += 256) {
+                    const f32x4 v = *(const f32x4_any*)(at + i);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) take(v[e]);
+                }
+                for (; i < j.length; i++) take(at[i]);
             }
-            for (; i < j.length; i++) m.add(at[i]);
-        }
+        };
+        Range m;
+        visit([&](float x) { m.add(x); });
         unsigned largest = m.most;
 #pragma unroll
         for (int step = 32; step > 0; step >>= 1) { const unsigned o = __shfl_xor(largest, step); largest = o > largest ? o : largest; }
-        const int low = __popcll(__ballot(m.far_below(largest))), some = __popcll(__ballot(m.most != 0));
-        if (lane == 0) j.out[row] = exponent_for(largest, low, some);
+        const unsigned bound = small_bound(largest);
+        unsigned small = m.below(bound);
+        if (m.least[2] < bound) small = 0, visit([&](float x) { small += magnitude(x) - 1 < bound; });
+#pragma unroll
+        for (int step = 32; step > 0; step >>= 1) small += __shfl_xor(small, step);
+        if (lane == 0) j.out[row] = note_on(largest, small, elements);
         return;
     }
     // lane: 4 neighbouring rows c .. c + 3 of the block's 32, stretch 8 wave + lane / 8
-    __shared__ unsigned waves_largest[8][32];
-    __shared__ unsigned waves_low[8][8], waves_some[8][8];          // counts of 4 rows, a byte each
+    __shared__ unsigned waves_largest[8][32], waves_small[8][32];
     const int q = lane & 7, c = (int)block * 32 + q * 4, first = wave * 8 + (lane >> 3);
+    const auto visit = [&](auto take) {
+        for (int k = 0; k < 2; k++) {
+            if (!j.p[k]) continue;
+            if (c + 4 <= j.count) {
+                const float* const at = j.p[k] + c;
+                int l = first;
+                for (; l + 7 * 64 < j.length; l += 8 * 64) {                 // eight requests on their way
+                    f32x4 v[8];
+#pragma unroll
+                    for (int u = 0; u < 8; u++) v[u] = *(const f32x4_any*)(at + (int64_t)(l + u * 64) * j.ld);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int u = 0; u < 8; u++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) take(e, v[u][e]);
+                }
+                for (; l < j.length; l += 64) {
+                    const f32x4 v = *(const f32x4_any*)(at + (int64_t)l * j.ld);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) take(e, v[e]);
+                }
+            } else
+                for (int l = first; l < j.length; l += 64)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) if (c + e < j.count) take(e, j.p[k][(int64_t)l * j.ld + c + e]);
+        }
+    };
     Range m[4];
-    for (int k = 0; k < 2; k++) {
-        if (!j.p[k]) continue;
-        if (c + 4 <= j.count) {
-            const float* const at = j.p[k] + c;
-#pragma unroll 8
-            for (int l = first; l < j.length; l += 64) {
-                const f32x4 v = *(const f32x4_any*)(at + (int64_t)l * j.ld);
-#pragma unroll
-                for (int e = 0; e < 4; e++) m[e].add(v[e]);
-            }
-        } else
-            for (int l = first; l < j.length; l += 64)
-#pragma unroll
-                for (int e = 0; e < 4; e++) if (c + e < j.count) m[e].add(j.p[k][(int64_t)l * j.ld + c + e]);
-    }
+    visit([&](int e, float x) { m[e].add(x); });
     unsigned largest[4] = {m[0].most, m[1].most, m[2].most, m[3].most};
 #pragma unroll
     for (int step = 8; step < 64; step <<= 1)
@@ -398,24 +449,35 @@ __global__ __launch_bounds__(512) void operand_scales_kernel(const ScaleJobs job
 #pragma unroll
         for (int e = 0; e < 4; e++) waves_largest[wave][q * 4 + e] = largest[e];
     __syncthreads();
-    unsigned low = 0, some = 0;
+    unsigned bound[4], small[4];
+    bool look = false;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         for (int w = 0; w < 8; w++) { const unsigned o = waves_largest[w][q * 4 + e]; largest[e] = o > largest[e] ? o : largest[e]; }
-        low |= (unsigned)m[e].far_below(largest[e]) << (8 * e);
-        some |= (unsigned)(m[e].most != 0) << (8 * e);
+        bound[e] = small_bound(largest[e]);
+        small[e] = m[e].below(bound[e]);
+        look |= m[e].least[2] < bound[e];
+    }
+    if (look) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) small[e] = 0;
+        visit([&](int e, float x) { small[e] += magnitude(x) - 1 < bound[e]; });
     }
 #pragma unroll
-    for (int step = 8; step < 64; step <<= 1) { low += __shfl_xor(low, step); some += __shfl_xor(some, step); }
-    if (lane < 8) { waves_low[wave][q] = low; waves_some[wave][q] = some; }
+    for (int step = 8; step < 64; step <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; e++) small[e] += __shfl_xor(small[e], step);
+    if (lane < 8)
+#pragma unroll
+        for (int e = 0; e < 4; e++) waves_small[wave][q * 4 + e] = small[e];
     __syncthreads();
-    if (wave == 0 && lane < 8) {
-        low = some = 0;
-        for (int w = 0; w < 8; w++) { low += waves_low[w][q]; some += waves_some[w][q]; }
+    if (wave == 0 && lane < 8)
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (c + e < j.count) j.out[c + e] = exponent_for(largest[e], (low >> (8 * e)) & 255, (some >> (8 * e)) & 255);
-    }
+        for (int e = 0; e < 4; e++) {
+            unsigned all = 0;
+            for (int w = 0; w < 8; w++) all += waves_small[w][q * 4 + e];
+            if (c + e < j.count) j.out[c + e] = note_on(largest[e], all, elements);
+        }
 }
 
 __device__ __forceinline__ void lds_barrier() {             // orders LDS only: requests to memory stay in flight
@@ -438,17 +500,17 @@ struct SplitShare {
     int l_of;                                               // first l of the thread inside a slice
 
     __device__ __forceinline__ void place(const float* a, int64_t ld, int first, int count, int t, int half_of_columns, const float* other,
-                                          const int* exponents, const int* other_exponents) {
+                                          const int* notes, const int* other_notes) {
         // half_of_columns > 0: rows from there on belong to the second matrix of a pair
 #pragma unroll
         for (int u = 0; u < E / 4; u++) {
             int r = ALONG ? (t + u * THREADS) >> 2 : t % WIDTH;
             const float* from = a;
-            const int* exponent = exponents;
-            if (half_of_columns > 0 && r >= half_of_columns) { r -= half_of_columns; from = other; exponent = other_exponents; }
+            const int* note = notes;
+            if (half_of_columns > 0 && r >= half_of_columns) { r -= half_of_columns; from = other; note = other_notes; }
             const int64_t row = first + r < count ? first + r : count - 1;       // past the end: the last one, its results are not stored
             base[u] = from + row * (ALONG ? ld : 1);
-            if constexpr (PLANES == 2) scale[u] = __builtin_bit_cast(float, (unsigned)(exponent[row] + 127) << 23);
+            if constexpr (PLANES == 2) scale[u] = __builtin_bit_cast(float, (unsigned)(exponent_of(note[row]) + 127) << 23);
         }
         l_of = ALONG ? (t & 3) * 4 : __builtin_amdgcn_readfirstlane(t / WIDTH) * E;
     }
@@ -520,9 +582,9 @@ __device__ __forceinline__ void split_product_tile(const Product<float>& g, unsi
     typedef Partial<PLANES> Part;
     constexpr unsigned A_BYTES = PLANES * AShare::PLANE, BUFFER = A_BYTES + PLANES * BShare::PLANE;
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, wm = wave / WN, wn = wave % WN;
-    // exponent of the tile's row r, column c (columns of a pair: the first product's, then the second's)
-    const auto row_exponent = [&](int r) { return g.a_scale[m0 + r < g.rows ? m0 + r : g.rows - 1]; };
-    const auto column_exponent = [&](int c) {
+    // the note on the tile's row r, column c (columns of a pair: the first product's, then the second's)
+    const auto row_note = [&](int r) { return g.a_scale[m0 + r < g.rows ? m0 + r : g.rows - 1]; };
+    const auto column_note = [&](int c) {
         const int n = n0 + (PAIRED && c >= HALF ? c - HALF : c);
         return g.b_scale[PAIRED && c >= HALF][n < g.cols ? n : g.cols - 1];
     };
@@ -652,63 +714,144 @@ __device__ __forceinline__ void split_product_tile(const Product<float>& g, unsi
         }
     }
 
-    // (two planes: the slices' memory takes the exponents of the tile's rows and columns; every row in it is finite, and so is every sum)
-    int* const exponents = (int*)lds;
+    // (two planes: the slices' memory takes the notes on the tile's rows and columns; every row in it is finite, and so is every sum)
+    int* const notes = (int*)lds;
     if constexpr (PLANES == 2) {
-        for (int r = t; r < BM; r += THREADS) exponents[r] = row_exponent(r);
-        for (int c = t; c < BN; c += THREADS) exponents[BM + c] = column_exponent(c);
+        for (int r = t; r < BM; r += THREADS) notes[r] = row_note(r);
+        for (int c = t; c < BN; c += THREADS) notes[BM + c] = column_note(c);
         lds_barrier();
     }
-    // one fragment of the result (PAIRED: the same fragment of both products) to where it belongs.
-    // Register v of lane l: row 8 (v / 4) + 4 (l / 32) + v % 4, column l % 32 of the fragment.
+    // Register v of lane l: row 8 (v / 4) + 4 (l / 32) + v % 4, column l % 32 of a fragment.  Rows are counted from the tile's first, columns from
+    // that of one product's half.
+    const auto row_of = [&](int i, int v) { return (wm * FI + i) * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3); };
+    const auto columns_of = [&](int j) { return (PAIRED ? wn * (FJ / 2) + j : wn * FJ + j) * 32; };
     const int64_t shift = (int64_t)part * g.part_stride;
-    const auto write = [&](int i, int j, const f32x16& xs, const f32x16& ys) {
-        const int c = (PAIRED ? wn * (FJ / 2) + j : wn * FJ + j) * 32 + (lane & 31), n = n0 + c;
-        const int x_exponent = PLANES == 2 ? exponents[BM + c] : 0, y_exponent = PLANES == 2 && PAIRED ? exponents[BM + HALF + c] : 0;
-#pragma unroll
-        for (int v = 0; v < 16; v++) {
-            const int r = (wm * FI + i) * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3), m = m0 + r;
-            if (m >= g.rows || n >= g.cols) continue;
-            const int64_t at = (int64_t)m * g.cols + n + shift;
-            const float x = PLANES == 2 ? __builtin_ldexpf(xs[v], -(exponents[r] + x_exponent)) : xs[v];
-            const float y = !PAIRED ? 0.0f : PLANES == 2 ? __builtin_ldexpf(ys[v], -(exponents[r] + y_exponent)) : ys[v];
-            if constexpr (PAIRED && EPI == GATED) {
-                g.out[0][at] = gated_fun(g.fun, x) * y;
-                if (g.out[1]) { g.out[1][at] = x; g.out[2][at] = y; }
-            } else {
-                g.out[0][at] = x;
-                if constexpr (PAIRED) g.out[1][at] = y;
-            }
+    const auto put = [&](int r, int c, float x, float y) {
+        const int m = m0 + r, n = n0 + c;
+        if (m >= g.rows || n >= g.cols) return;
+        const int64_t at = (int64_t)m * g.cols + n + shift;
+        if constexpr (PAIRED && EPI == GATED) {
+            g.out[0][at] = gated_fun(g.fun, x) * y;
+            if (g.out[1]) { g.out[1][at] = x; g.out[2][at] = y; }
+        } else {
+            g.out[0][at] = x;
+            if constexpr (PAIRED) g.out[1][at] = y;
         }
     };
     constexpr int SHOWN = PAIRED ? FJ / 2 : FJ;             // fragments per row of the wavefront's tile, of one product
-    unsigned again = 0;                                     // fragments with a result that is not finite
+    unsigned again = 0;                                     // fragments with results to be computed again
+    unsigned* const open = (unsigned*)lds + BM + BN + wave * (FI * SHOWN * 64) + lane;        // two planes: which of the lane's, 64 words a fragment
+    static_assert((BM + BN + WM * WN * FI * SHOWN * 64) * 4 <= 2 * BUFFER, "notes and results to be computed again fit where the slices were");
 #pragma unroll
-    for (int i = 0; i < FI; i++)
+    for (int i = 0; i < FI; i++) {
+        int most_small = 0;                                 // of the lane's rows
+        if constexpr (PLANES == 2)
+#pragma unroll
+            for (int v = 0; v < 16; v++) { const int n = small_of(notes[row_of(i, v)]); most_small = n > most_small ? n : most_small; }
 #pragma unroll
         for (int j = 0; j < SHOWN; j++) {
             const f32x16 &x = acc[i][j], &y = acc[i][PAIRED ? FJ / 2 + j : j];
+            const int c = columns_of(j) + (lane & 31);
             if constexpr (PLANES == 3) {
                 bool odd = false;
 #pragma unroll
                 for (int v = 0; v < 16; v++) odd |= !(__builtin_fabsf(x[v]) < INFINITY) || !(__builtin_fabsf(y[v]) < INFINITY);
                 if (__any(odd)) { again |= 1u << (i * SHOWN + j); continue; }
+#pragma unroll
+                for (int v = 0; v < 16; v++) put(row_of(i, v), c, x[v], y[v]);
+            } else {
+                const int x_note = notes[BM + c], y_note = PAIRED ? notes[BM + HALF + c] : x_note;
+                float least = INFINITY;
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    least = __builtin_fminf(least, __builtin_fabsf(x[v]));
+                    if constexpr (PAIRED) least = __builtin_fminf(least, __builtin_fabsf(y[v]));
+                }
+                const int small = small_of(x_note) > small_of(y_note) ? small_of(x_note) : small_of(y_note);
+                unsigned uncertain = 0;
+                if (__any(least < UNCERTAIN * (float)(most_small + small))) {
+#pragma unroll
+                    for (int v = 0; v < 16; v++) {
+                        const int note = notes[row_of(i, v)];
+                        const bool bad = __builtin_fabsf(x[v]) < least_certain(note, x_note) || (PAIRED && __builtin_fabsf(y[v]) < least_certain(note, y_note));
+                        uncertain |= (unsigned)(bad && m0 + row_of(i, v) < g.rows && n0 + c < g.cols) << v;
+                    }
+                    if (__any(uncertain != 0)) { again |= 1u << (i * SHOWN + j); open[(i * SHOWN + j) * 64] = uncertain; }
+                }
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const int r = row_of(i, v), e = exponent_of(notes[r]);
+                    if (!(uncertain >> v & 1)) put(r, c, __builtin_ldexpf(x[v], -(e + exponent_of(x_note))), PAIRED ? __builtin_ldexpf(y[v], -(e + exponent_of(y_note))) : 0.0f);
+                }
             }
-            write(i, j, x, y);
         }
-    if constexpr (PLANES == 3)
+    }
+    // What has to be computed again, from the floats as they are.  A slice of the part's whole ones, then what is left of each segment:
+    const int turns = last - first + (last == all && g.inner % 16 != 0 ? g.segments : 0);
+    const auto slice_of = [&](int turn, int& segment) {      // its first l
+        const int s = first + turn, left = s - all;
+        segment = left >= 0 ? left : s >= whole;
+        return (left >= 0 ? whole : s - segment * whole) * 16;
+    };
 #pragma unroll 1
     for (int f = 0; f < FI * SHOWN; f++) {
         if (!(again >> f & 1)) continue;
         const int i = f / SHOWN, j = f % SHOWN;
-        const int m = m0 + (wm * FI + i) * 32 + (lane & 31), n = n0 + (PAIRED ? wn * (FJ / 2) + j : wn * FJ + j) * 32 + (lane & 31);
+        if constexpr (PLANES == 2) {
+            // Up to 8 results: one after the other, by all lanes together (a fragment takes the time of about ten).
+            unsigned mine = open[f * 64], count = __builtin_popcount(mine);
+#pragma unroll
+            for (int step = 32; step > 0; step >>= 1) count += __shfl_xor(count, step);
+            if (count <= 8) {
+                while (const uint64_t lanes = __ballot(mine != 0)) {
+                    const int owner = __builtin_ctzll(lanes), v = __builtin_ctz(__shfl(mine, owner));
+                    if (lane == owner) mine &= mine - 1;
+                    const int r = (wm * FI + i) * 32 + 8 * (v >> 2) + 4 * (owner >> 5) + (v & 3), c = columns_of(j) + (owner & 31);
+                    const int64_t am = (int64_t)(m0 + r) * (A_ALONG ? g.lda : 1), bn = (int64_t)(n0 + c) * (B_ALONG ? g.ldb : 1);
+                    float x = 0, y = 0;
+                    const auto add = [&](int segment, int from, int end) {
+                        const float *const ap = g.A[segment] + am, *const bp = g.B[PAIRED ? 0 : segment] + bn, *const cp = g.B[1] + bn;
+                        const int64_t a_step = A_ALONG ? 1 : g.lda, b_step = B_ALONG ? 1 : g.ldb;
+                        int l = from + lane;
+                        for (; l + 15 * 64 < end; l += 16 * 64) {            // 16 at a time on their way
+                            float av[16], bv[16], cv[16];
+#pragma unroll
+                            for (int u = 0; u < 16; u++) {
+                                av[u] = ap[(l + u * 64) * a_step];
+                                bv[u] = bp[(l + u * 64) * b_step];
+                                if constexpr (PAIRED) cv[u] = cp[(l + u * 64) * b_step];
+                            }
+#pragma unroll
+                            for (int u = 0; u < 16; u++) {
+                                x = __builtin_fmaf(av[u], bv[u], x);
+                                if constexpr (PAIRED) y = __builtin_fmaf(av[u], cv[u], y);
+                            }
+                        }
+                        for (; l < end; l += 64) {
+                            const float av = ap[l * a_step];
+                            x = __builtin_fmaf(av, bp[l * b_step], x);
+                            if constexpr (PAIRED) y = __builtin_fmaf(av, cp[l * b_step], y);
+                        }
+                    };
+                    for (int segment = 0; segment < g.segments; segment++) {
+                        const int from = first - segment * whole, end = last - segment * whole;
+                        add(segment, (from > 0 ? from : 0) * 16, (end < whole ? end : whole) * 16);
+                        if (last == all) add(segment, whole * 16, g.inner);
+                    }
+#pragma unroll
+                    for (int step = 32; step > 0; step >>= 1) { x += __shfl_xor(x, step); y += __shfl_xor(y, step); }
+                    if (lane == 0) put(r, c, x, y);
+                }
+                continue;
+            }
+        }
+        const int c = columns_of(j) + (lane & 31), m = m0 + (wm * FI + i) * 32 + (lane & 31), n = n0 + c;
         const int64_t am = (int64_t)(m < g.rows ? m : g.rows - 1) * (A_ALONG ? g.lda : 1), bn = (int64_t)(n < g.cols ? n : g.cols - 1) * (B_ALONG ? g.ldb : 1);
         f32x16 x = {}, y = {};
-        const int turns = last - first + (last == all && g.inner % 16 != 0 ? g.segments : 0);
 #pragma unroll 2
         for (int turn = 0; turn < turns; turn++) {
-            const int s = first + turn, left = s - all;
-            const int segment = left >= 0 ? left : s >= whole, l0 = (left >= 0 ? whole : s - segment * whole) * 16;
+            int segment;
+            const int l0 = slice_of(turn, segment);
             const float* const ap = g.A[segment] + am;
             const float* const bp = g.B[PAIRED ? 0 : segment] + bn;
 #pragma unroll
@@ -724,7 +867,8 @@ __device__ __forceinline__ void split_product_tile(const Product<float>& g, unsi
                 }
             }
         }
-        write(i, j, x, y);
+#pragma unroll
+        for (int v = 0; v < 16; v++) put(row_of(i, v), c, x[v], y[v]);
     }
 }
 
