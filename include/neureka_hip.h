@@ -268,8 +268,8 @@ int nk_layer_norm(nk_dev dev, int dtype, int64_t rows, int64_t cols, nk_buf src,
 int nk_layer_norm_backward(nk_dev dev, int dtype, int64_t rows, int64_t cols, nk_buf src, int64_t src_pitch, nk_buf gain, nk_buf mean,
                            nk_buf rstd, nk_buf error, nk_buf d_src, nk_buf d_gain, nk_buf d_bias);
 
-/* Dropout: drn[i] = keep(i) ? src[i] / (1 - probability) : 0 for every i of a view, n elements (drn may be src
- * with the same view).
+/* Dropout: drn[i] = keep(i) ? src[i] / (1 - probability) : 0 for every i of a view, n elements.  drn may be src
+ * with the same view; a drain that shares elements with its source in any other way, or holds an element twice along an axis, is refused.
  * keep(i): word i % 4 of Philox4x32-10 with key = seed and counter = (i / 4, offset) is at least floor(probability * 2^32), i the
  * row-major index.  No mask is stored: the backward pass is the same call on the error.  Calls that shall draw
  * independently differ in seed or offset. */

@@ -7,6 +7,7 @@
 // 32 x 32 -> 64-bit products, 60 further integer operations) run beside the memory traffic, which bounds the kernel: x in, y out
 // (4096 x 4096 floats 24 us, 5.6 TB/s).
 #include "nk_internal.h"
+#include "nk_views.h"
 
 namespace nk {
 
@@ -104,6 +105,25 @@ extern "C" int nk_dropout(nk_dev h, int dtype, int rank, nk_buf drn, const int32
     Cfg dc, sc;
     load_cfg(dc, drn_cfg, rank);
     load_cfg(sc, src_cfg, rank);
+    const auto view_of = [&](nk_buf at, const Cfg& c) {
+        View v;
+        v.first = (int64_t)(at / eb);
+        v.rank = rank;
+        for (int k = 0; k < rank; k++) {
+            v.first += (int64_t)c.offset[k] * c.strides[k];
+            v.extent[k] = c.shape[k];
+            v.step[k] = (int64_t)c.strides[k] * c.spread[k];
+        }
+        return v;
+    };
+    static_assert(View::MOST == NK_MAX_RANK, "a view has as many axes as a descriptor");
+    const View to = view_of(drn, dc), from = view_of(src, sc);
+    bool in_place = to.first == from.first;                 // (every element is read and written by the same thread)
+    for (int k = 0; k < rank; k++) {
+        NK_REQUIRE(to.extent[k] == 1 || to.step[k] != 0, "nk_dropout: axis %d of the drain holds one element %lld times", k, (long long)to.extent[k]);
+        in_place = in_place && (to.extent[k] == 1 || to.step[k] == from.step[k]);
+    }
+    NK_REQUIRE(in_place || !views_meet(to, from), "nk_dropout: the drain overlaps the source without being the same view of it");
     int64_t prod = 1;                                       // the mask follows the row-major index whatever table a view carries
     for (int k = rank - 1; k >= 0; k--) { dc.imap[k] = (int)prod; prod *= dc.shape[k]; }
     const Mask m = {(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)offset, (uint32_t)(offset >> 32), (uint64_t)(probability * 4294967296.0)};

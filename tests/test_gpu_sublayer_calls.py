@@ -1,0 +1,41 @@
+"""What the entry points of layerNorm, dropout and gatedMatMul take and refuse."""
+import numpy as np
+import pytest
+
+from test_gpu_sublayer import dropped, get, put
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dt", [np.float32, np.float64])
+def test_a_dropout_onto_a_part_of_its_own_source_is_refused(device, dt):
+    from neureka_amd import HipError
+    x = np.random.default_rng(1).standard_normal((64, 60)).astype(dt)
+    t = put(device, x)
+    square = t[0:60, 0:60]
+    for what, drain, source in (("shifted by a row", t[1:64, 0:60], t[0:63, 0:60]), ("shifted back", t[0:63, 0:60], t[1:64, 0:60]), ("by a column", t[0:64, 1:60], t[0:64, 0:59]),
+                                ("transposed", square.T(), square), ("a stride apart", t[0:32, 0:60], t[0:64:2, 0:60]), ("corners", t[0:40, 0:40], t[24:64, 20:60])):
+        with pytest.raises(HipError, match="overlaps"):
+            device.launch_dropout(drain, source, 0.5, 1)
+    assert get(t).tobytes() == x.tobytes()
+    (p, _, c), = device._ops(t)
+    twice = np.array([64, 60, 60, 0, 60, 1, 0, 0, 1, 1], np.int32)            # shape, strides (the columns all the same element), indices map, offset, spread
+    other = put(device, x)
+    lib = device._lib
+    assert lib.nk_dropout(device.handle, 0 if dt == np.float32 else 1, 2, other._data.ptr, twice.ctypes.data_as(type(c)), p, c, 0.5, 1, 0, 64 * 60) != 0
+    assert b"holds one element" in lib.nk_last_error()
+
+
+def test_a_dropout_between_parts_that_share_nothing_runs(device):
+    """Halves, alternating columns, a block and the transpose of its neighbour: in one buffer, with no element in common; in place."""
+    x = np.random.default_rng(2).standard_normal((64, 60)).astype(np.float32)
+    for drain, source in ((np.s_[0:64, 0:30], np.s_[0:64, 30:60]), (np.s_[0:64, 0:60:2], np.s_[0:64, 1:60:2]), (np.s_[0:32, 0:60], np.s_[32:64, 0:60]), (np.s_[0:64:2, 3:60], np.s_[1:64:2, 0:57]),
+                          (np.s_[5:64:3, 7:60:2], np.s_[5:64:3, 7:60:2])):
+        t, want = put(device, x), x.copy()
+        want[drain] = dropped(np.ascontiguousarray(x[source]), 7, 2, 0.3)
+        device.launch_dropout(t[drain], t[source], 0.3, 7, 2)
+        assert get(t).tobytes() == want.tobytes()
+    t, want = put(device, x), x.copy()
+    want[0:30, 0:30] = dropped(np.ascontiguousarray(x[0:30, 30:60].T), 7, 2, 0.3)
+    device.launch_dropout(t[0:30, 0:30], t[0:30, 30:60].T(), 0.3, 7, 2)
+    assert get(t).tobytes() == want.tobytes()
