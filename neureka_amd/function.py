@@ -32,8 +32,11 @@ def _device_for(inputs: Sequence[Tensor]):
     raise IllegalStateException("none of the operands is stored on a HipDevice; this package has no host arithmetic path")
 
 
-# operations whose operands keep their own ranks and whose gradients come out of one call
-SUBLAYER_OPERATIONS = ("layerNorm", "dropout", "gatedMatMul")
+# operations whose operands keep their own ranks and whose gradients come out of one call: the number of operands, the arguments by name
+# (those without a value have to be given)
+_REQUIRED = object()
+SUBLAYER_OPERATIONS = {"layerNorm": (3, {"epsilon": 1e-5}), "dropout": (1, {"probability": _REQUIRED, "seed": _REQUIRED, "offset": 0}),
+                       "gatedMatMul": (3, {"activation": "silu"})}
 
 
 def execute(op_id: str, inputs: Sequence[Tensor], d: int = -1, record: bool = True, args: Optional[dict] = None) -> Tensor:
@@ -69,9 +72,16 @@ def _execute_sublayer(operation, device, parents: Sequence[Tensor], d: int, reco
     """execute() for SUBLAYER_OPERATIONS: one algorithm each, which prepares ranks and views itself."""
     if d >= 0:
         raise IllegalArgumentException(f"'{operation.identifier}' has no elementwise derivative; its gradients come from backward()")
+    count, known = SUBLAYER_OPERATIONS[operation.identifier]
+    if len(parents) != count:
+        raise IllegalArgumentException(f"'{operation.identifier}' takes {count} operands, not {len(parents)}")
+    given = {**known, **args}
+    if len(given) != len(known) or _REQUIRED in given.values():
+        raise IllegalArgumentException(f"'{operation.identifier}' takes {', '.join(known)} by name, given: {', '.join(args) or 'none'}")
     wanted = [t._rqs_gradient or t._node is not None for t in parents]
     recorded = record and True in wanted
-    call = ExecutionCall(device, operation, list(parents), -1, operation.algorithms[0], dict(args, keep=recorded))
+    given["keep"] = recorded
+    call = ExecutionCall(device, operation, list(parents), -1, operation.algorithms[0], given)
     result = execute_on_common_device(call, lambda c: execute_device_algorithm(c.algorithm.prepare(c)))
     if recorded:
         result._node = GraphNode(parents, (), _joint_gradients(call, parents, wanted))
