@@ -109,7 +109,8 @@ def _joint_gradients(call: ExecutionCall, parents: Sequence[Tensor], wanted: Lis
     shape, dtype, parent_shapes = call.inputs[0].shape, call.inputs[0].dtype, [t.shape for t in parents]
 
     def act(error: Tensor) -> List[Optional[Tensor]]:
-        if error.shape != shape or error.dtype != dtype:
+        # (axes of one element may stand anywhere: an operand of lower rank was padded, and its error has the padded shape)
+        if error.dtype != dtype or (error.shape != shape and [n for n in error.shape if n > 1] != [n for n in shape if n > 1]):
             raise IllegalArgumentException(f"the error of a {dtype}{list(shape)} result cannot be {error.dtype}{list(error.shape)}")
         # operands that live on the host are stored for the launch and restored afterwards
         run = ExecutionCall(device, operation, operands + [error])
@@ -120,7 +121,11 @@ def _joint_gradients(call: ExecutionCall, parents: Sequence[Tensor], wanted: Lis
             error.setIsVirtual(False)
         out = [Tensor._on_device(device, dtype, s, zeroed=False) if w else None for s, w in zip(parent_shapes, wanted)]
         if op_id == "dropout":                    # the same mask on the error
-            device.launch_dropout(out[0], error, args["probability"], args["seed"], args["offset"])
+            drain = out[0]
+            if drain.shape != error.shape:        # seen in the error's shape
+                axes = iter([k for k, n in enumerate(drain.shape) if n > 1])
+                drain = drain.permute(*[next(axes) if n > 1 else -1 for n in error.shape])
+            device.launch_dropout(drain, error, args["probability"], args["seed"], args["offset"])
         elif op_id == "layerNorm":
             device.launch_layer_norm_backward(operands[0], operands[1], args["stats"], as_dense(error), *out)
         else:

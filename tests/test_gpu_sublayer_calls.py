@@ -39,3 +39,32 @@ def test_a_dropout_between_parts_that_share_nothing_runs(device):
     want[0:30, 0:30] = dropped(np.ascontiguousarray(x[0:30, 30:60].T), 7, 2, 0.3)
     device.launch_dropout(t[0:30, 0:30], t[0:30, 30:60].T(), 0.3, 7, 2)
     assert get(t).tobytes() == want.tobytes()
+
+
+@pytest.mark.parametrize("padded", [(1, 7, 12), (7, 12, 1), (7, 1, 12)])
+def test_gradients_of_padded_errors(device, padded):
+    """The same gradients, bit for bit, from an error that has further axes of one element, dense or a view."""
+    rng = np.random.default_rng(3)
+    x, g, w, e = (rng.standard_normal(s).astype(np.float32) for s in ((7, 12), (12,), (12, 12), (7, 12)))
+    tg, tw = put(device, g), put(device, w)
+    wide = np.full(tuple(n + 2 for n in padded), np.nan, np.float32)
+    wide[1:-1, 1:-1, 1:-1] = e.reshape(padded)
+    part = put(device, wide)[tuple(slice(1, n + 1) for n in padded)]
+    for f in (lambda t: t.layerNorm(tg, tg), lambda t: t.dropout(0.4, 5, 6), lambda t: t.gatedMatMul(tw, tw)):
+        seen = []
+        for error in (put(device, e), put(device, e.reshape(padded)), part):
+            t = put(device, x).setRqsGradient(True)
+            f(t).backward(error)
+            assert t.gradient.shape == (7, 12)
+            seen.append(get(t.gradient).tobytes())
+        assert seen[0] == seen[1] == seen[2]
+
+
+def test_a_norm_inside_a_residual_stream_of_higher_rank(device):
+    rng = np.random.default_rng(4)
+    x, g, b, r = (rng.standard_normal(s).astype(np.float32) for s in ((7, 12), (12,), (12,), (1, 7, 12)))
+    t = put(device, x).setRqsGradient(True)
+    (t.layerNorm(put(device, g), put(device, b)) * put(device, r)).backward(1.0)
+    alone = put(device, x).setRqsGradient(True)
+    alone.layerNorm(put(device, g), put(device, b)).backward(put(device, r[0]))
+    assert get(t.gradient).tobytes() == get(alone.gradient).tobytes()
