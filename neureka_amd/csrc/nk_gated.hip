@@ -1318,6 +1318,17 @@ static void launch_scales(Device* dev, const ScaleJobs& jobs) {
     hipLaunchKernelGGL(operand_scales_kernel, dim3(blocks), dim3(512), 0, dev->stream, jobs);
 }
 
+// What ran, for nk_last_path: f64 tiles, or those of two or three planes; split: the contraction in parts.
+static int tiles_name(size_t item, bool two) { return item == 8 ? 0 : two ? 1 : 2; }
+static const char* const TILES[3] = {"gated_tiles", "gated_tiles_two_planes", "gated_tiles_three_planes"};
+static const char* const TILES_SPLIT[3] = {"gated_tiles_split", "gated_tiles_two_planes_split", "gated_tiles_three_planes_split"};
+#define NK_BACKWARD_WITH(x) {"gated_backward" x, "gated_backward" x "_w_tiles", "gated_backward" x "_w_tiles_split", "gated_backward" x "_w_two_planes", \
+                             "gated_backward" x "_w_two_planes_split", "gated_backward" x "_w_three_planes", "gated_backward" x "_w_three_planes_split"}
+static const char* const BACKWARD[9][7] = {          // [d_X: not wanted, few rows, few rows split, then as the second][weights: not wanted, tiles, ...]
+    NK_BACKWARD_WITH(""), NK_BACKWARD_WITH("_x_few_rows"), NK_BACKWARD_WITH("_x_few_rows_split"), NK_BACKWARD_WITH("_x_tiles"), NK_BACKWARD_WITH("_x_tiles_split"),
+    NK_BACKWARD_WITH("_x_two_planes"), NK_BACKWARD_WITH("_x_two_planes_split"), NK_BACKWARD_WITH("_x_three_planes"), NK_BACKWARD_WITH("_x_three_planes_split")};
+#undef NK_BACKWARD_WITH
+
 template <typename T>
 static int gated_forward(Device* dev, int fun, bool along, int64_t M, int64_t K, int64_t N, const T* X, const T* Wg, const T* Wu, T* H, T* gate, T* up) {
     Product<T> g{};
@@ -1349,7 +1360,8 @@ static int gated_forward(Device* dev, int fun, bool along, int64_t M, int64_t K,
     }
     launch_product<T, true, GATED>(dev, g, s, true, along, (T*)ws);
     NK_HIP(hipGetLastError());
-    set_path(s.parts > 1 ? "gated_tiles_split" : "gated_tiles");
+    const int t = tiles_name(sizeof(T), two);
+    set_path(s.parts > 1 ? TILES_SPLIT[t] : TILES[t]);
     return NK_OK;
 }
 
@@ -1397,7 +1409,9 @@ static int gated_backward(Device* dev, int fun, bool along, int64_t M, int64_t K
     }
     if (dWg) launch_product<T, true, STORE>(dev, gw, sw, false, false, partial);
     NK_HIP(hipGetLastError());
-    set_path("gated_backward_tiles");
+    const int x = !dX ? 0 : is_few ? 1 + (few.parts > 1) : 3 + 2 * tiles_name(sizeof(T), two_x) + (sx.parts > 1);
+    const int w = !dWg ? 0 : 1 + 2 * tiles_name(sizeof(T), two_w) + (sw.parts > 1);
+    set_path(BACKWARD[x][w]);
     return NK_OK;
 }
 

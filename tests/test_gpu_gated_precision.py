@@ -124,6 +124,16 @@ def test_scales_within_a_row_that_undo_each_other(device, along, binades):
     check_forward(device, x, wg, wu, along)
 
 
+@pytest.mark.parametrize("along", [False, True])
+def test_a_product_that_is_not_split_into_parts(device, along):
+    rng = np.random.default_rng(4)
+    M, K, N = 2048, 1200, 4096
+    x, wg = hidden(rng, M, K, N, np.arange(3, K, 100), 2.0 ** 24)
+    wu = rng.standard_normal((K, N)).astype(np.float32)
+    wu[:, 17] = wg[:, 18]
+    check_forward(device, x, wg, wu, along)
+
+
 def test_empty_rows_and_columns_and_sparse_operands(device):
     """Rows and columns of zeros beside rows with small entries; operands with one entry in fifty, half of them 2^-22 of the rest."""
     rng = np.random.default_rng(5)

@@ -1,4 +1,4 @@
-"""What the entry points of layerNorm, dropout and gatedMatMul take and refuse."""
+"""What the entry points of layerNorm, dropout and gatedMatMul take and refuse, and which kernels a product runs."""
 import numpy as np
 import pytest
 
@@ -68,3 +68,33 @@ def test_a_norm_inside_a_residual_stream_of_higher_rank(device):
     alone = put(device, x).setRqsGradient(True)
     alone.layerNorm(put(device, g), put(device, b)).backward(put(device, r[0]))
     assert get(t.gradient).tobytes() == get(alone.gradient).tobytes()
+
+
+# which kernels the shapes of the other tests are meant to run: forward, d_X, the weights' gradients
+PATHS = {
+    np.float32: [((1, 3001, 1301), "few_rows_split", "few_rows_split", "three_planes"), ((20, 3001, 1301), "few_rows_split", "few_rows_split", "three_planes"),
+                 ((16, 64, 65), "few_rows", "few_rows", "three_planes"), ((17, 100, 48), "few_rows", "few_rows", "three_planes"),
+                 ((40, 500, 701), "few_rows", "few_rows_split", "three_planes"), ((64, 1501, 700), "few_rows_split", "few_rows_split", "three_planes"),
+                 ((33, 1700, 1600), "tiles_three_planes_split", "three_planes_split", "three_planes"), ((150, 50, 70), "tiles_three_planes", "three_planes", "three_planes"),
+                 ((2500, 64, 65), "tiles_three_planes", "three_planes", "three_planes_split"), ((300, 1000, 500), "tiles_three_planes_split", "three_planes_split", "three_planes"),
+                 ((1301, 1307, 1299), "tiles_two_planes_split", "two_planes_split", "two_planes_split"), ((1300, 1310, 1290), "tiles_two_planes_split", "two_planes_split", "two_planes_split"),
+                 ((4099, 500, 1100), "tiles_two_planes", "two_planes_split", "two_planes_split"), ((700, 3000, 1100), "tiles_two_planes_split", "two_planes_split", "two_planes"),
+                 ((1200, 1400, 1310), "tiles_two_planes_split", "two_planes_split", "two_planes_split"), ((1200, 2048, 1290), "tiles_two_planes_split", "two_planes_split", "two_planes"),
+                 ((1300, 1210, 1408), "tiles_two_planes_split", "two_planes_split", "two_planes_split"), ((2048, 1200, 4096), "tiles_two_planes", "two_planes_split", "two_planes")],
+    np.float64: [((1, 3001, 1301), "few_rows_split", "few_rows_split", "tiles"), ((16, 64, 65), "few_rows", "few_rows", "tiles"), ((40, 500, 701), "tiles_split", "tiles_split", "tiles"),
+                 ((150, 50, 70), "tiles", "tiles", "tiles"), ((513, 48, 192), "tiles", "tiles_split", "tiles_split"), ((300, 1000, 500), "tiles_split", "tiles_split", "tiles")]}
+
+
+@pytest.mark.parametrize("along", [False, True])
+@pytest.mark.parametrize("dt,shape,forward,d_x,weights", [(dt, *p) for dt, paths in PATHS.items() for p in paths])
+def test_which_kernels_a_product_runs(device, dt, shape, forward, d_x, weights, along):
+    from neureka_amd import _lib
+    M, K, N = shape
+    zeros = lambda *s: put(device, np.zeros(s, dt))
+    x, w, y, e = zeros(M, K), zeros(N, K).T() if along else zeros(K, N), zeros(M, N), zeros(M, N)
+    device.launch_gated_matmul("silu", y, x, w, w)
+    assert _lib.last_path() == "gated_" + forward
+    dx, dg, du = zeros(M, K), zeros(K, N), zeros(K, N)
+    for wanted, path in (((dx, dg, du), f"gated_backward_x_{d_x}_w_{weights}"), ((dx, None, None), f"gated_backward_x_{d_x}"), ((None, dg, du), f"gated_backward_w_{weights}")):
+        device.launch_gated_matmul_backward("silu", x, w, w, y, y, e, *wanted)
+        assert _lib.last_path() == path
