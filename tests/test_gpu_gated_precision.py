@@ -161,3 +161,20 @@ def test_rows_at_the_ends_of_the_range(device):
     wg[:, 40], wu[:, 41] = 0, 0
     wg[17, 40], wu[18, 41] = 2.0 ** 100, 2.0 ** 90
     check_forward(device, x, wg, wu)
+
+
+@pytest.mark.parametrize("exponent", [-100, -110, -114, -118, -122, -125])
+def test_three_planes_at_the_lower_end_of_the_range(device, exponent):
+    """Products that take three bfloat16 numbers: below 2^-110 the last of them ends at multiples of 2^-133, so an operand is off by at
+    most 2^-134, and every result by that times what it meets."""
+    from neureka_amd import _lib
+    rng = np.random.default_rng(7)
+    M, K, N = 150, 200, 100
+    x = (rng.standard_normal((M, K)) * 2.0 ** exponent).astype(np.float32)
+    w = (rng.standard_normal((K, N)) * 2.0 ** 100).astype(np.float32)
+    X, W = x.astype(np.float64), w.astype(np.float64)
+    for got in forward(device, x, w, w, False):
+        assert "three_planes" in _lib.last_path()
+        tol = (8 + 4 * np.sqrt(K)) * U * (np.abs(X) @ np.abs(W)) + 2.0 ** -134 * np.abs(W).sum(0)
+        bad = np.abs(got - X @ W) > tol
+        assert not bad.any(), (bad.sum(), (np.abs(got - X @ W) / tol).max())
