@@ -848,24 +848,38 @@ __device__ __forceinline__ void split_product_tile(const Product<float>& g, unsi
         const int c = columns_of(j) + (lane & 31), m = m0 + (wm * FI + i) * 32 + (lane & 31), n = n0 + c;
         const int64_t am = (int64_t)(m < g.rows ? m : g.rows - 1) * (A_ALONG ? g.lda : 1), bn = (int64_t)(n < g.cols ? n : g.cols - 1) * (B_ALONG ? g.ldb : 1);
         f32x16 x = {}, y = {};
-#pragma unroll 2
-        for (int turn = 0; turn < turns; turn++) {
+        struct Slice { float a[8], b[8], c[8]; };
+        const auto request = [&](Slice& k, int turn) {
             int segment;
             const int l0 = slice_of(turn, segment);
-            const float* const ap = g.A[segment] + am;
-            const float* const bp = g.B[PAIRED ? 0 : segment] + bn;
+            const float *const ap = g.A[segment] + am, *const bp = g.B[PAIRED ? 0 : segment] + bn, *const cp = g.B[1] + bn;
 #pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-                const int l = l0 + k + (lane >> 5);
+            for (int e = 0; e < 8; e++) {
+                const int l = l0 + 2 * e + (lane >> 5);
                 const bool in = l < g.inner;
                 const int64_t ao = (int64_t)(in ? l : 0) * (A_ALONG ? 1 : g.lda), bo = (int64_t)(in ? l : 0) * (B_ALONG ? 1 : g.ldb);
-                const float av = in ? ap[ao] : 0.0f, bv = in ? bp[bo] : 0.0f;
-                x = __builtin_amdgcn_mfma_f32_32x32x2f32(av, bv, x, 0, 0, 0);
-                if constexpr (PAIRED) {
-                    const float cv = in ? g.B[1][bn + bo] : 0.0f;
-                    y = __builtin_amdgcn_mfma_f32_32x32x2f32(av, cv, y, 0, 0, 0);
-                }
+                const float av = ap[ao], bv = bp[bo];
+                k.a[e] = in ? av : 0.0f;
+                k.b[e] = in ? bv : 0.0f;
+                if constexpr (PAIRED) { const float cv = cp[bo]; k.c[e] = in ? cv : 0.0f; }
             }
+        };
+        const auto multiply_floats = [&](const Slice& k) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                x = __builtin_amdgcn_mfma_f32_32x32x2f32(k.a[e], k.b[e], x, 0, 0, 0);
+                if constexpr (PAIRED) y = __builtin_amdgcn_mfma_f32_32x32x2f32(k.a[e], k.c[e], y, 0, 0, 0);
+            }
+        };
+        Slice one, two;                                      // a slice on its way while the other is multiplied; past the end: the last once more
+        request(one, 0);
+        for (int turn = 0; turn < turns; turn += 2) {
+            request(two, turn + 1 < turns ? turn + 1 : turns - 1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply_floats(one);
+            request(one, turn + 2 < turns ? turn + 2 : turns - 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (turn + 1 < turns) multiply_floats(two);
         }
 #pragma unroll
         for (int v = 0; v < 16; v++) put(row_of(i, v), c, x[v], y[v]);
