@@ -44,12 +44,13 @@ def check_forward(device, x, wg, wu, along=False):
         close(got, X @ W, np.abs(X) @ np.abs(W), x.shape[1], what)
 
 
-def check_backward(device, x, wg, wu, e):
+def check_backward(device, x, wg, wu, e, along=False):
     """With gate = up = 1 and the identity, dg = du = e: dX = e (Wg + Wu)^T, dWg = dWu = x^T e."""
     (M, K), N = x.shape, wg.shape[1]
     one = device.allocateFromOne(np.float32, M * N, 1.0)
     d_x, d_g, d_u = (put(device, np.zeros(s, np.float32)) for s in ((M, K), (K, N), (K, N)))
-    device.launch_gated_matmul_backward("idy", put(device, x), put(device, wg), put(device, wu), one, one, put(device, e), d_x, d_g, d_u)
+    weight = (lambda w: put(device, np.ascontiguousarray(w.T)).T()) if along else (lambda w: put(device, w))
+    device.launch_gated_matmul_backward("idy", put(device, x), weight(wg), weight(wu), one, one, put(device, e), d_x, d_g, d_u)
     X, G, V, E = (a.astype(np.float64) for a in (x, wg, wu, e))
     read = lambda t: t.items.reshape(t.shape)
     close(read(d_x), E @ (G + V).T, np.abs(E) @ (np.abs(G) + np.abs(V)).T, 2 * N, "dX")
@@ -110,6 +111,29 @@ def test_single_results_from_small_entries(device):
         w[np.ix_(at, columns)] = held
     check_forward(device, x, wg, wu)
     check_forward(device, x, wg, wu, along=True)
+
+
+def crossing(b, at, columns):
+    """b[:, columns] zero everywhere but at `at`."""
+    held = b[np.ix_(at, columns)]
+    b[:, columns] = 0
+    b[np.ix_(at, columns)] = held
+
+
+@pytest.mark.parametrize("along", [False, True])
+def test_single_results_from_small_entries_in_gradients(device, along):
+    rng = np.random.default_rng(8)
+    M, K, N = 1300, 1210, 1409
+    x, wg, wu, e = (rng.standard_normal(s).astype(np.float32) for s in ((M, K), (K, N), (K, N), (M, N)))
+    g, u = wg.T.copy(), wu.T.copy()
+    for w in (g, u):                                        # d_X: rows of e against columns of both weights' transposes
+        crossing(w, [3, 800, N - 1], [0, 33, 1000, K - 1])
+    e[np.ix_([1, 130, 131, M - 1], [3, 800, N - 1])] *= np.float32(2.0 ** -26)
+    check_backward(device, x, np.ascontiguousarray(g.T), np.ascontiguousarray(u.T), e, along)
+    x, e = rng.standard_normal((M, K)).astype(np.float32), rng.standard_normal((M, N)).astype(np.float32)
+    crossing(e, [7, 640, M - 1], [4, 500, N - 1])           # the weights' gradients: columns of x against columns of e
+    x[np.ix_([7, 640, M - 1], [2, 300, 301, K - 1])] *= np.float32(2.0 ** -26)
+    check_backward(device, x, wg, wu, e, along)
 
 
 @pytest.mark.parametrize("binades", [10, 16, 17, 18, 19, 20, 21, 22, 23])
