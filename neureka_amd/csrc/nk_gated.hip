@@ -1310,10 +1310,10 @@ static int launch_few(Device* dev, Product<T> g, const FewPlan& f, bool along, T
 }
 
 // Whether a product takes two planes.  They save three of six partial products (at 1.1e15 operations a second) and cost a launch that reads
-// both operands.  Forward in microseconds, two planes against three: 512 x 1024 x 1024 29.6 / 29.2, 1024^3 37 / 40,
-// 1111 x 1000 x 2500 68 / 100, 2048^3 144 / 222; 65 x 4096 x 4096, all weights, 74 / 64.
+// both operands and a look at every result.  Forward in microseconds, weights that no cache holds, two planes against three:
+// 512 x 1024 x 1024 33.7 / 29.2, 1024^3 40.4 / 38.8, 1111 x 1000 x 2500 73 / 97, 2048^3 153 / 208; 65 x 4096 x 4096, all weights, 92 / 63.
 template <typename T> static bool two_planes(int64_t rows, int64_t cols, int64_t inner) {
-    const double saved_us = 6.0 * rows * cols * inner / 1.1e9, cost_us = 6.0 + 4.0 * (rows + cols) * inner / 4.5e6;
+    const double saved_us = 6.0 * rows * cols * inner / 1.1e9, cost_us = 9.0 + 4.0 * (rows + cols) * inner / 4.5e6;
     return sizeof(T) == 4 && saved_us > cost_us;
 }
 // Whether M rows go to few_rows_kernel.  Above 32 rows it holds four row tiles per wavefront and is bound by its matrix instructions, of
