@@ -256,7 +256,7 @@ __global__ __launch_bounds__(256, 2) void product_kernel(const Product<double> g
 
 // ---- f32 products on the 16-bit matrix cores --------------------------------------------------------------------------
 // The 16-bit instructions do 16 times the work of the f32 one per cycle and add exact partial products in f32, so a product of
-// sums of 16-bit numbers costs less than the product of the floats they make up, at the same accuracy.  Two ways (PLANES):
+// sums of 16-bit numbers costs less than the product of the floats they make up, and loses no more on ordinary operands.  Two ways (PLANES):
 //
 // 3: bfloat16, any operands.  A float is the sum of three, each the rest of the ones before rounded to nearest: 3 x 8 bits hold its 24
 // (below 2^-110 the last leaves bfloat16's range: off by at most 2^-134).  The six largest of the nine partial products are added,
@@ -567,7 +567,7 @@ struct SplitShare {
 };
 
 // Three tile sizes: 256 x 256 (8 wavefronts of 128 x 64: 48 KiB of LDS reads for 48 matrix instructions of a slice), 256 x 128 and
-// 128 x 128.  4096^3 forward, two planes: 756 us, 1.09e15 operations on halves a second, 364 TFLOP/s of float products (the f32
+// 128 x 128.  4096^3 forward, two planes: 740-755 us, 1.1e15 operations on halves a second, 364-372 TFLOP/s of float products (the f32
 // instruction's peak is 157, a library's product of floats reaches 154).  The clock falls to 1.7 GHz under it with the matrix cores busy 61 %
 // of the cycles, as under any dense product of 16-bit numbers here (a library's product of bfloat16, 8192^3: 1.3e15); without the
 // requests to memory and the splitting the same loop takes 605 us.  Three planes: 1199 us.
@@ -919,7 +919,7 @@ __global__ __launch_bounds__(WM * WN * 64) void split_product_kernel(const Produ
 //
 // What the memory delivers depends on how the requests lie (weights that no cache holds):
 //  - Weights by row, in floats: one row tile reads 128 bytes of a row per wavefront (CW 2; 1 x 4096 x 4096 28 us, 64 bytes 34).  Two row
-//    tiles and more read 64 and one chunk at a time (32 x 2048 x 3500 28 us, 128 bytes 35), four because the rest does not fit their registers.
+//    tiles and more read 64 and one chunk at a time (32 x 2048 x 3500 28 us, 128 bytes 35; four row tiles were measured this way alone).
 //  - Weights stored along l: 128 bytes per column (U 2; 16 x 4096 x 4096 26 us, U 1 31); four row tiles take one chunk (64 x 2048 x
 //    2048 19 us, U 2 24).  There every group starts at another place of the contraction, because groups that walk in step meet in the
 //    same memory channels (33 us in step, 28 apart).

@@ -5,7 +5,7 @@
 //     with the error e of y and g = e gain:
 //     dx = rstd (g - sum g / D - h sum (g h) / D)      dgain = sum over rows of e h      dbias = sum over rows of e
 //
-// A row is read once: it stays in the registers of its group of threads (a wavefront up to 1024 floats, a block of 256 or
+// A row is read once: it stays in the registers of its group of threads (a wavefront up to 512 floats, a block of 256 or
 // 1024 threads above) while its mean, then the sum of the squared distances from it, are formed; the variance is never
 // a difference of two large sums.  A block keeps its columns' gain (and bias) in registers and walks over rows with the next row
 // already requested.  The backward pass keeps the columns' share of dgain and dbias in registers as well and writes one
@@ -162,7 +162,8 @@ __global__ __launch_bounds__(BLOCK) void norm_backward_kernel(const NormArgs<T> 
         mean = a.mean[row]; rstd = a.rstd[row];
     }
     const T count = T(a.cols);
-    // a block of 1024 threads has 128 registers per thread: with four vectors of a row each, the next row does not fit beside this one
+    // a block of 1024 threads has 128 registers per thread: with four vectors of a row each, the next row does not fit beside this one (doubles
+    // spill 38 registers even so)
     constexpr bool AHEAD = BLOCK < 1024 || NV < 4;
     for (int turn = 0; row < a.rows; row += step, turn ^= 1) {
         V x_next[AHEAD ? NV : 1], err_next[AHEAD ? NV : 1];
@@ -315,7 +316,7 @@ __global__ __launch_bounds__(1024) void norm_add_shares_kernel(const T* __restri
 }
 
 // ---- plans ----------------------------------------------------------------------------------------------------------
-// Calls `f.template operator()<BLOCK, THREADS, NV>()` for the narrowest group of threads that holds a row; false: none does.
+// Calls `f.template operator()<BLOCK, THREADS, NV>()` for the narrowest of the groups of threads, a wavefront or a block, that holds a row; false: none does.
 template <typename T, typename F>
 static bool with_row_plan(int64_t cols, const F& f) {
     const int64_t vecs = (cols + Wide<T>::N - 1) / Wide<T>::N;
